@@ -20,7 +20,7 @@ and of recordings up to some forty minutes.
 
 The 4 bits: blocks of 32 consecutive dims of one token and head share a power
 of two 2^e, the smallest with max|x| <= 7 * 2^e (e kept in [-23, 13] for f16
-activations and in [-64, 125] for the others); x / 2^e, as a 32-bit number, is
+activations and in [-64, 64] for the others); x / 2^e, as a 32-bit number, is
 rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with its sign, ties to the
 value whose last bit is even, at most 6.
 """
@@ -203,7 +203,7 @@ LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
 
 def _exponent_range(dt):
-    return (-23, 13) if dt == torch.float16 else (-64, 125)
+    return (-23, 13) if dt == torch.float16 else (-64, 64)
 
 
 def _encode(x, dt):
