@@ -18,8 +18,10 @@ from .decoder import (  # noqa: F401
     Qwen3,
     Result,
     TextConfig,
+    TokenScores,
     lib,
 )
+from .paged import PAGE_TOKENS, PagedKvCache, Scored, generate_paged  # noqa: F401
 from . import transcript  # noqa: F401
 from .encoder import (  # noqa: F401
     WHISPER_MEDIUM,

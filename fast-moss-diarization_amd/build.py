@@ -24,11 +24,15 @@ SOURCES = [
     "rowops.hip",
     "attn_decode.hip",
     "attn_prefill.hip",
+    "pkv_rows.hip",
+    "pkv_attn.hip",
+    "logprobs.hip",
     "weights.hip",
     "encoder_kernels.hip",
     "fmd_dec.cpp",
     "encoder.cpp",
     "forward.cpp",
+    "pkv.cpp",
     "engine.cpp",
 ]
 
@@ -68,7 +72,7 @@ def _compile(src: str) -> Path:
 # register the compiler may otherwise use itself, so the device assembly of
 # these files is checked after every build: M0 may appear only in that
 # block's `s_mov_b32 m0, sN`, with the global_load_lds two lines below.
-LDS_COPY_SOURCES = ["gemm.hip", "attn_prefill.hip", "encoder_kernels.hip"]
+LDS_COPY_SOURCES = ["gemm.hip", "attn_prefill.hip", "encoder_kernels.hip", "pkv_attn.hip"]
 
 
 def _device_asm(src: str) -> str:

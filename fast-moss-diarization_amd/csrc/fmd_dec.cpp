@@ -51,6 +51,7 @@ int DevBuf::ensure(size_t bytes, bool* fresh) {
   if (bytes == 0) bytes = 256;
   if (hipMalloc(&p, bytes) != hipSuccess) {
     p = nullptr;
+    (void)hipGetLastError();   // reported here: the next launch's check must not find it
     return fmd_fail(FMD_ERR_OOM, "device allocation of " + std::to_string(bytes) + " bytes failed");
   }
   n = bytes;

@@ -50,12 +50,12 @@ struct DecodeLane {
 // Per-handle device scratch, sized on demand (never inside a graph capture).
 struct Workspace {
   DevBuf x, xn, qkv, q, ctx, act, logits, amax, pml, po, ids, pad, rowmeta, tiles, lastx, embeds,
-      done, ntok, finish, tokens, force, gstate, opstate, oppad, asrc, audio;
+      done, ntok, finish, tokens, force, gstate, opstate, oppad, asrc, audio, lastrow, score, lpwork;
   DecodeLane dec;
   void release_all() {
     for (DevBuf* b : {&x, &xn, &qkv, &q, &ctx, &act, &logits, &amax, &pml, &po, &ids, &pad,
                       &rowmeta, &tiles, &lastx, &embeds, &done, &ntok, &finish, &tokens, &force,
-                      &gstate, &opstate, &oppad, &asrc, &audio})
+                      &gstate, &opstate, &oppad, &asrc, &audio, &lastrow, &score, &lpwork})
       b->release();
     dec.release_all();
   }
@@ -86,6 +86,7 @@ struct fmd_dec {
   std::vector<int32_t> op_pad;
   int op_len = -1;
   int logits_rows = 0;  // rows of the last logits launch (prefill / decode step), 0 = none
+  int score_rows = 0;   // rows of ws.logits that fmd_dec_logprobs reads, 0 = none
   const void* op_state_buf = nullptr;
   const void* op_pad_buf = nullptr;
   // Polls of one wait in the single-launch attention before it gives up and
@@ -110,6 +111,11 @@ struct fmd_kv {
   std::vector<void*> k, v;
   int32_t* state = nullptr;  // device: [0] length, [1] greedy step, [2] rows done
 };
+
+// The launches of one layer over the current plan of a paged cache (pkv.cpp).
+int pkv_append(fmd_pkv* c, int layer, const void* qkv, void* q);
+int pkv_attention(fmd_pkv* c, int layer, const void* q, void* ctx);
+fmd_dec* pkv_dec(const fmd_pkv* c);
 
 int kv_sync_state(fmd_kv* kv);
 // Resolves and clears the no-allocation attention's static scratch of

@@ -3,6 +3,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "pkv_pages.h"
+
 // Activation dtype codes (the activation dtype of each precision, precision.rs:32-41).
 enum ActDtype { ACT_F32 = 0, ACT_F16 = 1, ACT_BF16 = 2 };
 // Weight storage kinds.
@@ -270,3 +272,69 @@ hipError_t launch_enc_attn(int act, const EncAttnArgs& a, int heads, int windows
 // Number of argmax partial keys the EPI_LOGITS projection writes per row.
 // Work-groups (= argmax partials per row) of the EPI_LOGITS projection.
 int gemv_logits_nparts(int act, bool q8, bool norm, int hidden, int out_rows);
+
+// ---- paged 4-bit KV cache (pkv_rows.hip, pkv_attn.hip; layouts in pkv_pages.h) ----
+
+struct PkvRowArgs {
+  const int32_t* plan;
+  int layer, nh, nkv;
+  int rows;              // rows of the caller's buffers: rows past it are left alone
+  const void* x;         // append: (rows, (nh + 2 nkv) hd); write: K (rows, nkv, hd)
+  const void* v;         // write: V (rows, nkv, hd)
+  const void* qn_w;      // append
+  const void* kn_w;
+  const void* cos;
+  const void* sin;
+  float eps;
+  void* q_out;           // append: (rows, nh, hd)
+  void* k_out;           // read
+  void* v_out;
+};
+hipError_t launch_pkv_append(int act, const PkvRowArgs& a, hipStream_t s);
+hipError_t launch_pkv_write(int act, const PkvRowArgs& a, hipStream_t s);
+hipError_t launch_pkv_read(int act, const PkvRowArgs& a, hipStream_t s);
+
+// Page copies: page src[i] to page dst[i] in every layer, pairs by value.
+constexpr int kPkvPairs = 448;
+struct PkvPairs {
+  int32_t src[kPkvPairs], dst[kPkvPairs];
+};
+hipError_t launch_pkv_copy(const PkvPairs& p, int n, int layers, int nkv, const void* src_pool,
+                           int src_pages, void* dst_pool, int dst_pages, hipStream_t s);
+hipError_t launch_pkv_clear_plan(int32_t* plan, hipStream_t s);
+
+struct PkvAttnArgs {
+  const int32_t* plan;
+  int layer, nkv, rep;
+  int rows;              // rows of the caller's buffers
+  const void* q;         // (rows, nh, hd)
+  void* out;             // (rows, nh, hd)
+  int window, sinks;     // window 0: every key up to the query's own
+  float scale;
+  int ndec, ndseq, npre, nsplit;   // the plan's counts when the call was made
+  int captured;          // into a graph, whose replays may need joins that this plan does not
+  float* dec_ml;         // (slots, nkv, rep, 2)
+  float* dec_o;          // (slots, nkv, rep, hd)
+  float* pre_ml;         // (slots, nkv, tile rows, 2)
+  float* pre_o;          // (slots, nkv, tile rows, hd)
+};
+hipError_t launch_pkv_attn(int act, const PkvAttnArgs& a, hipStream_t s);
+// Query positions of a many-token tile (its rows are these times rep).
+int pkv_tile_positions(int act, int rep);
+
+// ---- log probabilities (logprobs.hip) ----
+struct LogprobArgs {
+  const void* x;         // (rows, vocab) in dtype (0 f32, 1 f16, 2 bf16), row stride ld
+  int64_t ld;
+  int dtype, rows, vocab;
+  const int32_t* target; // (rows) or NULL
+  int top;
+  float* logp;           // (rows) or NULL
+  float* entropy;        // (rows) or NULL
+  int32_t* ids;          // (rows, top)
+  float* best;           // (rows, top)
+  void* work;            // logprob_work_bytes()
+};
+int logprob_max_top();
+size_t logprob_work_bytes();   // enough for every call
+hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s);

@@ -802,6 +802,7 @@ int prefill_impl(fmd_dec* d, fmd_kv* kv, const void* emb_dev, const int32_t* pad
   CHK(launch_logits(d, w.lastx.p, B, w.logits.as<float>(), s));
   kv->len = total;
   d->logits_rows = B;
+  d->score_rows = B;
   return 0;
 }
 
@@ -864,6 +865,7 @@ int generate_group(fmd_dec* d, const void* emb_src, int on_dev, const int32_t* p
   if (!rc && timed) timed = hipEventRecord(ev[0], d->stream) == hipSuccess;
   if (!rc) rc = prefill_impl(d, kv, emb, pad, B, total, chunk);
   if (!rc && timed) timed = hipEventRecord(ev[1], d->stream) == hipSuccess;
+  d->score_rows = 0;   // the loop's logits are not left for a caller
   if (!rc) rc = setup_greedy(d, kv, B, budget, force);
   if (!rc) {
     // greedy step 0 on the prefill logits
@@ -930,6 +932,7 @@ extern "C" int fmd_dec_decode_step(fmd_dec* d, fmd_kv* kv, const uint32_t* ids, 
   CHK(decode_layers(d, kv, B, w.pad.as<int32_t>(), nullptr, d->stream));
   kv->len += 1;
   d->logits_rows = B;
+  d->score_rows = B;
   if (logits)
     HIPCHK(hipMemcpyAsync(logits, w.logits.p, (size_t)B * d->V * 4, hipMemcpyDeviceToHost, d->stream));
   HIPCHK(hipStreamSynchronize(d->stream));
@@ -988,6 +991,7 @@ extern "C" int fmd_dec_decode_loop(fmd_dec* d, fmd_kv* kv, const uint32_t* first
   HIPCHK(hipMemcpyAsync(w.ids.p, first_ids, (size_t)B * 4, hipMemcpyHostToDevice, d->stream));
   LAUNCH(launch_embed(d->act, w.ids.as<uint32_t>(), B, d->embed, d->H, w.x.p, d->stream));
   CHK(setup_greedy(d, kv, B, budget, force));
+  d->score_rows = 0;
   int steps = 0;
   CHK(run_decode_steps(d, kv, B, max_steps, budget, force != nullptr, eos, &steps));
   if (steps_run) *steps_run = steps;
@@ -1187,6 +1191,224 @@ extern "C" int fmd_op_logits(fmd_dec* d, const void* x, int rows, float* logits)
                         kMaxDecodeRows * 8));
   CHK(launch_logits(d, x, rows, logits, d->stream));
   HIPCHK(hipStreamSynchronize(d->stream));
+  return 0;
+}
+
+// ---------------------------------------------------------------------------
+// Steps over the paged 4-bit cache, and the scores of the last logits.
+
+namespace {
+
+// Every layer over the plan's `rows` rows in ws.x: the products of up to 16
+// rows by the GEMVs with the norms in their prologues, those of more by the
+// GEMMs.
+int paged_layers(fmd_dec* d, fmd_pkv* c, int rows) {
+  Workspace& w = d->ws;
+  hipStream_t s = d->stream;
+  const int act = d->act;
+  const bool few = rows <= kMaxDecodeRows;
+  auto gemm = [&](int epi, const void* x, const LinWeights& W, void* y, int ldy, const void* resid) {
+    GemmArgs g{};
+    g.x = x;
+    g.ldx = W.in;
+    g.W = W;
+    g.M = rows;
+    g.y = y;
+    g.ldy = ldy;
+    g.resid = resid;
+    return launch_gemm(act, epi, g, s);
+  };
+  for (int l = 0; l < d->L; ++l) {
+    Layer& ly = d->layers[l];
+    if (few) {
+      LAUNCH(launch_gemv(act, EPI_STORE, true,
+                         gemv_args(w.x.p, d->H, ly.in_norm, d->eps, ly.qkv.w, rows, w.qkv.p, d->qkvd,
+                                   nullptr, nullptr), s));
+    } else {
+      LAUNCH(launch_rmsnorm(act, w.x.p, d->H, ly.in_norm, rows, d->H, d->eps, w.xn.p, d->H, s));
+      LAUNCH(gemm(EPI_STORE, w.xn.p, ly.qkv.w, w.qkv.p, d->qkvd, nullptr));
+    }
+    CHK(pkv_append(c, l, w.qkv.p, w.q.p));
+    CHK(pkv_attention(c, l, w.q.p, w.ctx.p));
+    if (few) {
+      LAUNCH(launch_gemv(act, EPI_RESID, false,
+                         gemv_args(w.ctx.p, d->qd, nullptr, d->eps, ly.o.w, rows, w.x.p, d->H, w.x.p,
+                                   nullptr), s));
+      LAUNCH(launch_gemv(act, EPI_SWIGLU, true,
+                         gemv_args(w.x.p, d->H, ly.post_norm, d->eps, ly.gate_up.w, rows, w.act.p, d->I,
+                                   nullptr, nullptr), s));
+      LAUNCH(launch_gemv(act, EPI_RESID, false,
+                         gemv_args(w.act.p, d->I, nullptr, d->eps, ly.down.w, rows, w.x.p, d->H, w.x.p,
+                                   nullptr), s));
+    } else {
+      LAUNCH(gemm(EPI_RESID, w.ctx.p, ly.o.w, w.x.p, d->H, w.x.p));
+      LAUNCH(launch_rmsnorm(act, w.x.p, d->H, ly.post_norm, rows, d->H, d->eps, w.xn.p, d->H, s));
+      LAUNCH(gemm(EPI_SWIGLU, w.xn.p, ly.gate_up.w, w.act.p, d->I, nullptr));
+      LAUNCH(gemm(EPI_RESID, w.act.p, ly.down.w, w.x.p, d->H, w.x.p));
+    }
+  }
+  return 0;
+}
+
+int paged_forward(fmd_dec* d, fmd_pkv* c, int n, const int32_t* counts, int rows, const uint32_t* ids,
+                  const void* embeds, int on_dev, float* logits) {
+  Workspace& w = d->ws;
+  hipStream_t s = d->stream;
+  CHK(w.x.ensure((size_t)rows * d->H * d->esz));
+  CHK(w.xn.ensure((size_t)rows * std::max(d->H, d->I) * d->esz));
+  CHK(w.qkv.ensure((size_t)rows * d->qkvd * d->esz));
+  CHK(w.q.ensure((size_t)rows * d->qd * d->esz));
+  CHK(w.ctx.ensure((size_t)rows * d->qd * d->esz));
+  CHK(w.act.ensure((size_t)rows * d->I * d->esz));
+  CHK(w.lastx.ensure((size_t)n * d->H * d->esz));
+  CHK(w.lastrow.ensure((size_t)n * 4));
+  CHK(w.logits.ensure((size_t)n * d->V * 4));
+  CHK(w.amax.ensure((size_t)gemv_logits_nparts(d->act, d->quant, true, d->H, d->V) * kMaxDecodeRows * 8));
+  d->logits_rows = d->score_rows = 0;
+  if (ids) {
+    CHK(w.ids.ensure((size_t)rows * 4));
+    HIPCHK(hipMemcpyAsync(w.ids.p, ids, (size_t)rows * 4, hipMemcpyHostToDevice, s));
+    LAUNCH(launch_embed(d->act, w.ids.as<uint32_t>(), rows, d->embed, d->H, w.x.p, s));
+  } else {
+    HIPCHK(hipMemcpyAsync(w.x.p, embeds, (size_t)rows * d->H * d->esz,
+                          on_dev ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice, s));
+  }
+  CHK(paged_layers(d, c, rows));
+  const void* last = w.x.p;
+  if (rows > n) {
+    std::vector<int32_t> at(n);
+    for (int i = 0, r = 0; i < n; ++i) at[i] = (r += counts[i]) - 1;
+    HIPCHK(hipMemcpyAsync(w.lastrow.p, at.data(), (size_t)n * 4, hipMemcpyHostToDevice, s));
+    LAUNCH(launch_gather_rows(d->act, w.x.p, d->H, w.lastrow.as<int32_t>(), n, d->H, w.lastx.p, d->H, s));
+    last = w.lastx.p;
+  }
+  for (int i = 0; i < n; i += kMaxDecodeRows)
+    CHK(launch_logits(d, (const char*)last + (size_t)i * d->H * d->esz, std::min(kMaxDecodeRows, n - i),
+                      w.logits.as<float>() + (size_t)i * d->V, s));
+  d->logits_rows = n <= kMaxDecodeRows ? n : 0;
+  d->score_rows = n;
+  if (logits)
+    HIPCHK(hipMemcpyAsync(logits, w.logits.p, (size_t)n * d->V * 4, hipMemcpyDeviceToHost, s));
+  HIPCHK(hipStreamSynchronize(s));
+  return 0;
+}
+
+int logprob_args(fmd_dec* d, const void* x, int dtype, int rows, int vocab, int64_t ld, int top,
+                 LogprobArgs* out) {
+  if (dtype < FMD_DT_F32 || dtype > FMD_DT_BF16) return fmd_fail(FMD_ERR_ARG, "bad dtype");
+  if (rows < 0 || rows > (1 << 20) || vocab < 1 || vocab > (1 << 28) || ld < vocab)
+    return fmd_fail(FMD_ERR_ARG, "rows must be in [0, 2^20], vocab in [1, 2^28], the row stride at least vocab");
+  if (top < 0 || top > logprob_max_top() || top > vocab)
+    return fmd_fail(FMD_ERR_ARG, "alternatives must be in [0, " + std::to_string(logprob_max_top()) +
+                                     "] and at most the vocabulary");
+  if (!d->ws.lpwork.p) {
+    // one size for every call: captured graphs keep its address
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    HIPCHK(hipStreamIsCapturing(d->stream, &cap));
+    if (cap != hipStreamCaptureStatusNone)
+      return fmd_fail(FMD_ERR_STATE, "the first call of a handle allocates: make one before capturing");
+    CHK(d->ws.lpwork.ensure(logprob_work_bytes()));
+  }
+  LogprobArgs a{};
+  a.x = x;
+  a.ld = ld;
+  a.dtype = dtype;
+  a.rows = rows;
+  a.vocab = vocab;
+  a.top = top;
+  a.work = d->ws.lpwork.p;
+  *out = a;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" int fmd_dec_step(fmd_dec* d, fmd_pkv* c, int n, const int32_t* seqs, const int32_t* counts,
+                            const uint32_t* ids, const void* embeds, int on_dev, float* logits) {
+  if (!d || !c) return fmd_fail(FMD_ERR_ARG, "null handle");
+  if (pkv_dec(c) != d) return fmd_fail(FMD_ERR_STATE, "cache belongs to another decoder");
+  if (!fmd_dec_ready(d)) return fmd_fail(FMD_ERR_STATE, "decoder weights are incomplete");
+  if (n < 1 || !seqs || !counts) return fmd_fail(FMD_ERR_ARG, "a step needs at least one sequence");
+  if (!ids == !embeds) return fmd_fail(FMD_ERR_ARG, "a step takes token ids or embeddings");
+  int64_t rows = 0;
+  for (int i = 0; i < n; ++i) {
+    if (counts[i] < 1) return fmd_fail(FMD_ERR_ARG, "a step needs a token of every sequence");
+    rows += counts[i];
+  }
+  if (rows > INT32_MAX) return fmd_fail(FMD_ERR_ARG, "too many new tokens");
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIPCHK(hipStreamIsCapturing(d->stream, &cap));
+  if (cap != hipStreamCaptureStatusNone) return fmd_fail(FMD_ERR_STATE, "a step cannot be captured");
+  for (int64_t i = 0; ids && i < rows; ++i)
+    if (ids[i] >= (uint32_t)d->V) return fmd_fail(FMD_ERR_ARG, "token id out of range");
+  CHK(fmd_pkv_plan(c, n, seqs, counts));   // refuses more rows than the cache was made for
+  const int rc = paged_forward(d, c, n, counts, (int)rows, ids, embeds, on_dev, logits);
+  if (rc) {
+    // the sequences are as long as before
+    const std::string keep = fmd_last_error();
+    for (int i = 0; i < n; ++i) (void)fmd_pkv_truncate(c, seqs[i], fmd_pkv_len(c, seqs[i]) - counts[i]);
+    return fmd_fail(rc, keep);
+  }
+  return 0;
+}
+
+extern "C" int fmd_op_logprobs(fmd_dec* d, const void* x, fmd_dtype dtype, int rows, int vocab,
+                               int64_t ld, const int32_t* targets, int top, float* logp,
+                               float* entropy, int32_t* top_ids, float* top_logp) {
+  if (!d) return fmd_fail(FMD_ERR_ARG, "null handle");
+  if ((rows > 0 && !x) || (logp && !targets && rows > 0) || (top > 0 && (!top_ids || !top_logp)))
+    return fmd_fail(FMD_ERR_ARG, "null argument");
+  if ((uintptr_t)x % (dtype == FMD_DT_F32 ? 4 : 2)) return fmd_fail(FMD_ERR_ARG, "unaligned logits");
+  HIPCHK(hipSetDevice(d->device));
+  LogprobArgs a;
+  CHK(logprob_args(d, x, dtype, rows, vocab, ld, top, &a));
+  if (rows == 0) return 0;
+  a.target = targets;
+  a.logp = logp;
+  a.entropy = entropy;
+  a.ids = top_ids;
+  a.best = top_logp;
+  LAUNCH(launch_logprobs(a, d->stream));
+  if (d->stream == d->own_stream) {
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    HIPCHK(hipStreamIsCapturing(d->stream, &cap));
+    if (cap == hipStreamCaptureStatusNone) HIPCHK(hipStreamSynchronize(d->stream));
+  }
+  return 0;
+}
+
+extern "C" int fmd_dec_logprobs(fmd_dec* d, int n, const uint32_t* tokens, int top, float* logp,
+                                float* entropy, uint32_t* top_ids, float* top_logp) {
+  if (!d) return fmd_fail(FMD_ERR_ARG, "null handle");
+  if (n < 1 || (logp && !tokens) || (top > 0 && (!top_ids || !top_logp)))
+    return fmd_fail(FMD_ERR_ARG, "null argument or empty batch");
+  if (d->score_rows != n)
+    return fmd_fail(FMD_ERR_STATE, "no logits for this batch: call prefill, decode_step or step first");
+  for (int i = 0; tokens && i < n; ++i)
+    if (tokens[i] >= (uint32_t)d->V) return fmd_fail(FMD_ERR_ARG, "token id out of range");
+  HIPCHK(hipSetDevice(d->device));
+  LogprobArgs a;
+  CHK(logprob_args(d, d->ws.logits.p, FMD_DT_F32, n, d->V, d->V, top, &a));
+  // tokens | logp | entropy | ids | best
+  CHK(d->ws.score.ensure((size_t)n * (3 + 2 * (size_t)top) * 4));
+  int32_t* base = d->ws.score.as<int32_t>();
+  hipStream_t s = d->stream;
+  if (tokens) {
+    HIPCHK(hipMemcpyAsync(base, tokens, (size_t)n * 4, hipMemcpyHostToDevice, s));
+    a.target = base;
+    a.logp = (float*)(base + n);
+  }
+  a.entropy = (float*)(base + 2 * (size_t)n);
+  a.ids = base + 3 * (size_t)n;
+  a.best = (float*)(a.ids + (size_t)n * top);
+  LAUNCH(launch_logprobs(a, s));
+  if (logp) HIPCHK(hipMemcpyAsync(logp, a.logp, (size_t)n * 4, hipMemcpyDeviceToHost, s));
+  if (entropy) HIPCHK(hipMemcpyAsync(entropy, a.entropy, (size_t)n * 4, hipMemcpyDeviceToHost, s));
+  if (top > 0) {
+    HIPCHK(hipMemcpyAsync(top_ids, a.ids, (size_t)n * top * 4, hipMemcpyDeviceToHost, s));
+    HIPCHK(hipMemcpyAsync(top_logp, a.best, (size_t)n * top * 4, hipMemcpyDeviceToHost, s));
+  }
+  HIPCHK(hipStreamSynchronize(s));
   return 0;
 }
 

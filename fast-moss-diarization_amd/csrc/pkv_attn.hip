@@ -1,0 +1,672 @@
+// Attention over the paged 4-bit KV cache: causal, with an optional sliding
+// window whose first tokens (the sinks) stay visible.
+//
+// A query at position p sees the keys j <= p with j > p - window or j < sinks
+// (window 0: every j <= p), its own among them, so no row is empty.
+//   ctx = sum_j softmax_j(q . k_j / sqrt(128)) v_j
+// in one pass over the keys with a running maximum m and sum l; scores, m, l
+// and the sums over v are 32 bits.
+//
+// One new token (a decode step) is bound by the cache's bytes, 136 per key and
+// KV head.  A wave takes whole pages: K codes go to registers, V codes by
+// direct-to-LDS copies, the next page's in flight while this one is computed.
+// - S^T = K q^T by 16x16x32 MFMAs: lane (c, g) = (l % 16, l / 16) of tile mt
+//   holds row c of the A operand, which is token 16 (c/4) + 4 mt + c%4, and of
+//   it the dims of block g, whose scale is then one per lane:
+//   v_cvt_scalef32_pk turns two codes into two scaled 16-bit values, exactly.
+//   The rows are picked so that a lane's 16 scores are tokens 16 g .. 16 g + 15.
+// - The heads of a KV group fill 1, 2 or 4 of the MFMA's 16 columns; the others
+//   carry what would otherwise take more instructions.  Column c is head c %
+//   REP, block (c / REP) % 4 of V's dims and term c / (4 REP): each column's
+//   p_j is multiplied by its V block's scale (the scale is along the sum's
+//   tokens and so cannot be an operand's own), and its terms split that product
+//   into bf16 parts, hi + lo, so that p keeps 16 bits where rounding to bf16
+//   alone keeps 8 (32-bit activations: three terms, 24 bits).
+// - O^T += V^T P^T with V's codes transposed by LDS 4-bit transpose reads (lane
+//   = dim, 16 tokens in 8 bytes) and widened without a scale.
+// The units' pages are cut into items so that a launch fills the device; a
+// second kernel joins the items of a row.
+//
+// Many new tokens (prefill) are bound by the products and the softmax.  A
+// work-group holds the queries of a tile, waves own (head, 16 QS positions);
+// each page is widened once into 16-bit K and V blocks in LDS (double
+// buffered, the next page's codes in registers meanwhile).
+#include <algorithm>
+#include <type_traits>
+
+#include "fmd_common.h"
+#include "fmd_kernels.h"
+
+namespace {
+
+constexpr int HD = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGrow = 8.f;   // log2 units that a row's scores may exceed its reference m by
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Two codes (byte SEL of w) times the power of two sc, as 16-bit values.
+template <bool F16, int SEL>
+__device__ __forceinline__ uint32_t widen2(uint32_t w, float sc) {
+  if constexpr (F16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, sc, SEL));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, SEL));
+}
+template <bool F16>
+__device__ __forceinline__ u32x4 widen8(uint32_t w, float sc) {
+  return u32x4{widen2<F16, 0>(w, sc), widen2<F16, 1>(w, sc), widen2<F16, 2>(w, sc),
+               widen2<F16, 3>(w, sc)};
+}
+template <bool F16>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (F16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+__device__ __forceinline__ float rd_bf16(float v) { return rd<ACT_BF16>(v); }
+
+// Eight activation values at p as NT bf16 (16-bit activations: one operand in
+// their own type) terms that add up to them.
+template <int A, int NT>
+__device__ __forceinline__ void load_terms(const void* q, size_t at, bool ok, u32x4* t) {
+  if constexpr (A != ACT_F32) {
+    t[0] = ok ? *(const u32x4*)((const uint16_t*)q + at) : u32x4{0, 0, 0, 0};
+  } else {
+    f32x4 a[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (ok) {
+      a[0] = *(const f32x4*)((const float*)q + at);
+      a[1] = *(const f32x4*)((const float*)q + at + 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float x = a[i >> 1][2 * (i & 1)], y = a[i >> 1][2 * (i & 1) + 1];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        t[n][i] = pack2<false>(x, y);
+        x -= rd_bf16(x);
+        y -= rd_bf16(y);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ const uint8_t* pool_of(const int32_t* plan) {
+  return (const uint8_t*)(((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL]);
+}
+
+// ---- one new token --------------------------------------------------------
+
+constexpr int kDecWaves = 4;
+
+template <int A, int REP>
+__global__ void __launch_bounds__(64 * kDecWaves) pkv_decode_kernel(PkvAttnArgs a) {
+  constexpr bool F16 = A == ACT_F16;
+  constexpr int NT = A == ACT_F32 ? 3 : 1;          // terms of q
+  constexpr int PT = A == ACT_F32 ? 3 : 2;          // terms of p
+  constexpr int TPP = 4 / REP;                      // terms that the columns of one MFMA hold
+  constexpr int PASSES = (PT + TPP - 1) / TPP;
+  constexpr int VB = 4096;                          // V codes of a page and head
+  __shared__ __attribute__((aligned(1024))) uint8_t sV[kDecWaves][2][VB];
+  __shared__ float sM[kDecWaves][REP], sL[kDecWaves][REP];
+  float* const sO = (float*)&sV[0][0][0];           // [wave][REP][HD], after the loop
+  const int32_t* plan = a.plan;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int head = blockIdx.y, nh = a.nkv * REP;
+  const int blk = (c / REP) & 3, term = c / (4 * REP);
+  const float c2 = a.scale * kLog2e;
+  const int n_items = plan[PH_NDEC];
+  const size_t stride = (size_t)a.nkv * kPkvHeadBytes;       // bytes of a page
+  const uint8_t* layer = pool_of(plan) + (size_t)a.layer * plan[PH_PAGES] * stride +
+                         (size_t)head * kPkvHeadBytes;
+  const uint32_t lv = lds_addr(sV[w]);
+  // V copy: instruction j brings tokens 16 j .. 16 j + 15; token t's 16-byte
+  // chunk x lies at chunk x ^ ((t / 4) % 4), so that a transpose read's 16
+  // tokens fall in distinct banks
+  uint32_t vsrc[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int t = 16 * j + (lane >> 2);
+    vsrc[j] = (uint32_t)(t * 64 + (((lane & 3) ^ ((t >> 2) & 3)) << 4));
+  }
+  const uint32_t ksrc = (uint32_t)((16 * (c >> 2) + (c & 3)) * 64 + 16 * g);   // + 256 mt
+
+  for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
+    const PkvDecItem item = ((const PkvDecItem*)(plan + PH_WORDS))[it];
+    if (item.row >= a.rows) continue;
+    const int32_t* table = plan + item.table;
+    auto page_of = [&](int v) { return v < item.sp ? v : item.wp + (v - item.sp); };
+    u32x4 qf[4][NT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      load_terms<A, NT>(a.q, ((size_t)item.row * nh + head * REP + c % REP) * HD + 32 * g + 8 * j, true,
+                        qf[j]);
+    f32x4 o[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m2 = -INFINITY, mr = 0.f, l = 0.f;   // mr: m2, or 0 while no key was seen
+
+    u32x4 kn[4], vsn;
+    uint32_t ksn = 0;
+    // id: the page to fetch, read one step ahead of its use
+    auto id_of = [&](int v) { return v < item.v1 ? table[page_of(v)] : 0; };
+    auto fetch = [&](int id, int buf) {
+      const uint8_t* page = layer + (size_t)__builtin_amdgcn_readfirstlane(id) * stride;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        lds_copy16(page + kPkvV, vsrc[j], lv + buf * VB + j * 1024);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) kn[mt] = *(const u32x4*)(page + ksrc + 256 * mt);
+      ksn = *(const uint32_t*)(page + kPkvKs + 4 * (16 * g + c));
+      vsn = *(const u32x4*)(page + kPkvVs + 64 * blk + 16 * g);
+    };
+    int buf = 0, id = id_of(item.v0 + w + kDecWaves);
+    if (item.v0 + w < item.v1) fetch(id_of(item.v0 + w), 0);
+    for (int v = item.v0 + w; v < item.v1; v += kDecWaves, buf ^= 1) {
+      u32x4 k[4], vs = vsn;
+      const uint32_t ks = ksn;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) k[mt] = kn[mt];
+      // this page's registers and V codes are there, and the reads of the buffer
+      // that the next page's go to are done
+      __builtin_amdgcn_s_waitcnt(0x70);   // vmcnt(0) lgkmcnt(0)
+      asm volatile("" ::: "memory");
+      if (v + kDecWaves < item.v1) {
+        fetch(id, buf ^ 1);
+        id = id_of(v + 2 * kDecWaves);
+      }
+
+      const int kb = page_of(v) * kPkvPage;
+      f32x4 s[4];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const float sc = __builtin_bit_cast(float, ((ks >> (8 * mt)) & 0xffu) << 23);
+        s[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x4 kf = widen8<F16>(k[mt][j], sc);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) s[mt] = mfma<F16>(kf, qf[j][n], s[mt]);
+        }
+      }
+      // tokens 16 g + 4 mt + i of the page
+      const bool full = kb + kPkvPage - 1 <= item.pos &&
+                        (a.window == 0 || kb > item.pos - a.window || kb + kPkvPage <= a.sinks);
+      if (!full) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int j = kb + 16 * g + e;
+          if (j > item.pos || (a.window != 0 && j <= item.pos - a.window && j >= a.sinks))
+            s[e >> 2][e & 3] = -INFINITY;
+        }
+      }
+      float bm = s[0][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) bm = fmaxf(bm, s[e >> 2][e & 3]);
+      if (__any(fmaf(bm, c2, -mr) > kGrow || m2 == -INFINITY)) {
+        bm = fmaxf(bm, __shfl_xor(bm, 16));
+        bm = fmaxf(bm, __shfl_xor(bm, 32));
+        const float mn = fmaxf(m2, bm * c2), nr = mn == -INFINITY ? 0.f : mn;
+        const float f = __builtin_amdgcn_exp2f(m2 - nr);
+        m2 = mn;
+        mr = nr;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[d] *= f;
+      }
+      // p' = p * 2^(scale - 127): one exponential each, so that a masked
+      // token's p' is 0 whatever its scale byte is
+      float p[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float x = fmaf(s[e >> 2][e & 3], c2, -mr);
+        l += __builtin_amdgcn_exp2f(x);
+        const uint32_t byte = (vs[e >> 2] >> (8 * (e & 3))) & 0xffu;
+        p[e] = __builtin_amdgcn_exp2f(x + ((float)byte - 127.f));
+      }
+      const uint8_t* vb = &sV[w][buf][0];
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+      u32x4 pf[PASSES][2];
+#pragma unroll
+      for (int ps = 0; ps < PASSES; ++ps)
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          float x = p[e], y = p[e + 1];
+          // the column's term of the split: 0 the value, 1 what rounding left ..
+          const int tt = ps * TPP + term;
+#pragma unroll
+          for (int n = 1; n < PT; ++n) {
+            if (ps * TPP + TPP - 1 < n) break;   // no column of this pass has it
+            const float rx = rd_bf16(x), ry = rd_bf16(y);
+            if (tt >= n) {
+              x -= rx;
+              y -= ry;
+            }
+          }
+          if ((ps + 1) * TPP > PT && tt >= PT) x = y = 0.f;
+          pf[ps][e >> 3][(e & 7) >> 1] = pack2<false>(x, y);
+        }
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        // 16 tokens of dim 16 d + c: lane c of group g names token 16 g + c's
+        // 8 bytes of dims 16 d ..
+        const int t = 16 * g + c;
+        const i32x2 vt = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (lds_i32x2*)(vb + t * 64 + (((d >> 1) ^ ((t >> 2) & 3)) << 4) + 8 * (d & 1)));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x4 vf = widen8<false>((uint32_t)vt[h], 1.f);
+#pragma unroll
+          for (int ps = 0; ps < PASSES; ++ps) o[d] = mfma<false>(vf, pf[ps][h], o[d]);
+        }
+      }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    // the terms of a column add up; dims 32 b .. come from block b's columns
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = o[d][i];
+        if constexpr (REP == 1) x += __shfl_xor(x, 4);
+        if constexpr (REP <= 2) x += __shfl_xor(x, 8);
+        o[d][i] = x;
+      }
+    __syncthreads();   // every wave has read its V codes
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+      if (c < 4 * REP && blk == d >> 1)
+        *(f32x4*)&sO[(w * REP + c % REP) * HD + 16 * d + 4 * g] = o[d];
+    if (c < REP && g == 0) {
+      sM[w][c] = m2;
+      sL[w][c] = l;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < REP * HD; i += 64 * kDecWaves) {
+      const int r = i / HD, d = i % HD;
+      float M = sM[0][r];
+#pragma unroll
+      for (int j = 1; j < kDecWaves; ++j) M = fmaxf(M, sM[j][r]);
+      const float R = M == -INFINITY ? 0.f : M;
+      float L = 0.f, x = 0.f;
+#pragma unroll
+      for (int j = 0; j < kDecWaves; ++j) {
+        // a wave without pages has m = -inf, l = 0 and o = 0
+        const float f = __builtin_amdgcn_exp2f(sM[j][r] - R);
+        L += f * sL[j][r];
+        x += f * sO[(j * REP + r) * HD + d];
+      }
+      if (item.slot < 0) {
+        ((typename ActT<A>::T*)a.out)[((size_t)item.row * nh + head * REP + r) * HD + d] = st_act<A>(x / L);
+      } else {
+        const size_t u = ((size_t)item.slot * a.nkv + head) * REP + r;
+        a.dec_o[u * HD + d] = x;
+        if (d == 0) {
+          a.dec_ml[2 * u] = M;
+          a.dec_ml[2 * u + 1] = L;
+        }
+      }
+    }
+    __syncthreads();   // before the next item's copies overwrite sO
+  }
+}
+
+// Joins the items of each row: one work-group per (sequence, KV head).
+template <int A, int REP>
+__global__ void __launch_bounds__(REP * HD) pkv_decode_join_kernel(PkvAttnArgs a) {
+  const int32_t* plan = a.plan;
+  const int head = blockIdx.y, r = threadIdx.x / HD, d = threadIdx.x % HD;
+  for (int s = blockIdx.x; s < plan[PH_NDSEQ]; s += gridDim.x) {
+    const PkvDecSeq q = ((const PkvDecSeq*)(plan + plan[PH_DSEQ]))[s];
+    if (q.n < 2 || q.row >= a.rows) continue;
+    auto unit = [&](int i) { return ((size_t)(q.first + i) * a.nkv + head) * REP + r; };
+    float M = -INFINITY;
+    for (int i = 0; i < q.n; ++i) M = fmaxf(M, a.dec_ml[2 * unit(i)]);
+    const float R = M == -INFINITY ? 0.f : M;
+    float L = 0.f, x = 0.f;
+    for (int i = 0; i < q.n; ++i) {
+      const size_t u = unit(i);
+      const float f = __builtin_amdgcn_exp2f(a.dec_ml[2 * u] - R);
+      L += f * a.dec_ml[2 * u + 1];
+      x += f * a.dec_o[u * HD + d];
+    }
+    ((typename ActT<A>::T*)a.out)[((size_t)q.row * a.nkv * REP + head * REP + r) * HD + d] = st_act<A>(x / L);
+  }
+}
+
+// ---- many new tokens --------------------------------------------------------
+
+// Waves of a work-group and sets of 16 positions of a wave.
+template <int A, int REP> struct PreShape {
+  static constexpr int QS = A == ACT_F32 ? 1 : 2;
+  static constexpr int NW = REP == 1 ? 4 : 8;
+  static constexpr int TP = 16 * QS * (NW / REP);   // positions of a tile
+};
+
+__device__ __forceinline__ int swk(int t) { return t & 15; }
+__device__ __forceinline__ int swv(int t) { return (t & 7) << 1; }
+
+template <int A, int REP>
+__global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kernel(PkvAttnArgs a) {
+  constexpr bool F16 = A == ACT_F16;
+  constexpr int NT = A == ACT_F32 ? 3 : 1;     // terms of q and of p
+  constexpr int QS = PreShape<A, REP>::QS, NW = PreShape<A, REP>::NW, TP = PreShape<A, REP>::TP;
+  constexpr int NTH = 64 * NW, CH = 512 / NTH; // 16-byte chunks of codes per thread and page
+  constexpr int BLK = kPkvPage * HD;
+  __shared__ __attribute__((aligned(16))) uint16_t sK[2][BLK];
+  __shared__ __attribute__((aligned(16))) uint16_t sV[2][BLK];
+  const int32_t* plan = a.plan;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int qr = lane & 15, kg = lane >> 4;
+  const int r = w % REP, half = w / REP, nh = a.nkv * REP;
+  const float c2 = a.scale * kLog2e;
+  const size_t stride = (size_t)a.nkv * kPkvHeadBytes;
+  const int n_units = plan[PH_NPRE] * a.nkv;
+  const uint8_t* pool = pool_of(plan) + (size_t)a.layer * plan[PH_PAGES] * stride;
+
+  for (int un = blockIdx.x; un < n_units; un += gridDim.x) {
+    // Adjacent items of a KV head (a sequence's tiles) read the same pages:
+    // each XCD (work-groups are dealt round-robin) takes a contiguous run.
+    int unit = un;
+    {
+      const int per = n_units >> 3;
+      if (un < 8 * per) unit = (un & 7) * per + (un >> 3);
+    }
+    const int head = unit / plan[PH_NPRE];
+    const PkvPreItem item = ((const PkvPreItem*)(plan + plan[PH_PITEM]))[unit % plan[PH_NPRE]];
+    const int rows = min(item.n, a.rows - item.row);
+    if (rows <= 0) continue;
+    const int h = head * REP + r;
+    const int32_t* table = plan + item.table;
+    const uint8_t* hbase = pool + (size_t)head * kPkvHeadBytes;
+    auto page_of = [&](int v) { return v < item.sp ? v : item.wp + (v - item.sp); };
+    const int last = item.pos + item.n - 1;      // the tile's last position
+
+    int lim[QS];
+    u32x4 qf[QS][4][NT];
+    float m2[QS], mr[QS];
+    f32x4 o[QS][8], ls[QS];
+#pragma unroll
+    for (int qs = 0; qs < QS; ++qs) {
+      const int my = 16 * (QS * half + qs) + qr;
+      const bool ok = my < rows;
+      lim[qs] = ok ? item.pos + my : item.pos;   // rows past the end see what the first does
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        load_terms<A, NT>(a.q, ((size_t)(item.row + my) * nh + h) * HD + 32 * ks + 8 * kg, ok, qf[qs][ks]);
+      m2[qs] = -INFINITY;
+      mr[qs] = 0.f;
+      ls[qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int d = 0; d < 8; ++d) o[qs][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const uint32_t one2 = pack2<F16>(1.f, 1.f);
+    const u32x4 ones = u32x4{one2, one2, one2, one2};
+
+    // Codes of chunk x of a page (x < 256: K, else V): token (x / 4) % 64, block x % 4.
+    u32x4 raw[CH];
+    int rsc[CH];
+    auto fetch = [&](int v) {
+      const uint8_t* hp = hbase + (size_t)table[page_of(v)] * stride;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int x = i * NTH + tid, t = (x >> 2) & 63, b = x & 3;
+        raw[i] = *(const u32x4*)(hp + 16 * x);
+        rsc[i] = hp[x < 256 ? kPkvKs + 64 * b + 4 * (4 * (t >> 4) + (t & 3)) + ((t >> 2) & 3)
+                            : kPkvVs + 64 * b + t];
+      }
+    };
+    // Widened into LDS.  K's NaN scale makes the token's scores NaN; V's values
+    // are kept finite (they meet p = 0 of the rows that do not see the token),
+    // and what lies past the last visible token, which no one may have
+    // written, is 0.
+    auto stage = [&](int v, int buf) {
+      const int kb = page_of(v) * kPkvPage;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int x = i * NTH + tid, t = (x >> 2) & 63, b = x & 3;
+        const bool isv = x >= 256;
+        int byte = rsc[i];
+        if (isv && byte == 255) byte = 127;
+        const float sc = __builtin_bit_cast(float, (uint32_t)byte << 23);
+        const bool dead = kb + t > last;
+        uint16_t* row = (isv ? sV[buf] : sK[buf]) + t * HD;
+        const int sw = isv ? swv(t) : swk(t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          u32x4 e = widen8<F16>(raw[i][j], sc);
+          if (dead) e = u32x4{0, 0, 0, 0};
+          *(u32x4*)(row + (((4 * b + j) ^ sw) << 3)) = e;
+        }
+      }
+    };
+    if (item.v0 < item.v1) {
+      fetch(item.v0);
+      stage(item.v0, 0);
+    }
+    __syncthreads();
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    for (int v = item.v0, buf = 0; v < item.v1; ++v, buf ^= 1) {
+      const bool more = v + 1 < item.v1;
+      if (more) fetch(v + 1);
+      const int kb = page_of(v) * kPkvPage;
+      const uint16_t* kbuf = sK[buf];
+      const uint16_t* vbuf = sV[buf];
+      f32x4 s[4][QS];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) s[mt][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const int t = 16 * mt + qr;
+          const u32x4 ka = *(const u32x4*)(kbuf + t * HD + (((4 * ks + kg) ^ swk(t)) << 3));
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[mt][qs] = mfma<F16>(ka, qf[qs][ks][n], s[mt][qs]);
+        }
+      }
+      const bool full = kb + kPkvPage - 1 <= item.pos &&
+                        (a.window == 0 || kb > last - a.window || kb + kPkvPage <= a.sinks);
+      bool grow = false;
+      float bm[QS];
+#pragma unroll
+      for (int qs = 0; qs < QS; ++qs) {
+        if (!full) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int j = kb + 16 * (e >> 2) + 4 * kg + (e & 3);
+            if (j > lim[qs] || (a.window != 0 && j <= lim[qs] - a.window && j >= a.sinks))
+              s[e >> 2][qs][e & 3] = -INFINITY;
+          }
+        }
+        bm[qs] = s[0][qs][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) bm[qs] = fmaxf(bm[qs], s[e >> 2][qs][e & 3]);
+        grow |= fmaf(bm[qs], c2, -mr[qs]) > kGrow || m2[qs] == -INFINITY;
+      }
+      if (__any(grow)) {
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+          float x = fmaxf(bm[qs], __shfl_xor(bm[qs], 16));
+          x = fmaxf(x, __shfl_xor(x, 32));
+          const float mn = fmaxf(m2[qs], x * c2), nr = mn == -INFINITY ? 0.f : mn;
+          const float f = __builtin_amdgcn_exp2f(m2[qs] - nr);
+          m2[qs] = mn;
+          mr[qs] = nr;
+          ls[qs] *= f;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) o[qs][d] *= f;
+        }
+      }
+      // O^T += V^T P^T over tokens 32 hb .. 32 hb + 31: k-slot i of group kg is
+      // token 32 hb + 4 kg + i (i < 4) or 32 hb + 16 + 4 kg + i - 4, where S^T has them
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) {
+        u32x4 pb[QS][NT];
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const f32x4 x = s[2 * hb + (e >> 2)][qs];
+            float p0 = __builtin_amdgcn_exp2f(fmaf(x[e & 3], c2, -mr[qs]));
+            float p1 = __builtin_amdgcn_exp2f(fmaf(x[(e & 3) + 1], c2, -mr[qs]));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              pb[qs][n][e / 2] = pack2<F16>(p0, p1);
+              if (n + 1 < NT) {
+                p0 -= rd_bf16(p0);
+                p1 -= rd_bf16(p1);
+              }
+            }
+          }
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) ls[qs] = mfma<F16>(ones, pb[qs][n], ls[qs]);
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const int t = 32 * hb + 4 * kg + (qr >> 2);
+          const uint16_t* at = vbuf + t * HD + (((2 * d + ((qr & 3) >> 1)) ^ swv(t)) << 3) + 4 * (qr & 1);
+          const s16x4 r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+          const s16x4 r2 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * HD));
+          const u32x4 va = __builtin_bit_cast(u32x4, __builtin_shufflevector(r1, r2, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[qs][d] = mfma<F16>(va, pb[qs][n], o[qs][d]);
+        }
+      }
+      if (more) stage(v + 1, buf ^ 1);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int qs = 0; qs < QS; ++qs) {
+      const int my = 16 * (QS * half + qs) + qr;
+      if (my >= rows) continue;
+      if (item.slot < 0) {
+        const float inv = 1.f / ls[qs][0];
+        const size_t at = ((size_t)(item.row + my) * nh + h) * HD + 4 * kg;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          const f32x4 x = o[qs][d] * inv;
+          if constexpr (A == ACT_F32) {
+            *(f32x4*)((float*)a.out + at + 16 * d) = x;
+          } else {
+            uint32_t* p = (uint32_t*)((uint16_t*)a.out + at + 16 * d);
+            p[0] = pack2<F16>(x[0], x[1]);
+            p[1] = pack2<F16>(x[2], x[3]);
+          }
+        }
+      } else {
+        const size_t u = ((size_t)item.slot * a.nkv + head) * (TP * REP) + my * REP + r;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) *(f32x4*)(a.pre_o + u * HD + 16 * d + 4 * kg) = o[qs][d];
+        if (kg == 0) {
+          a.pre_ml[2 * u] = m2[qs];
+          a.pre_ml[2 * u + 1] = ls[qs][0];
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Joins the items of the tiles that were cut: a work-group per (8 query rows,
+// KV head), 32 lanes and 4 dims each to a row.
+template <int A, int REP>
+__global__ void __launch_bounds__(256) pkv_prefill_join_kernel(PkvAttnArgs a) {
+  constexpr int TR = PreShape<A, REP>::TP * REP, GR = TR / 8;
+  const int32_t* plan = a.plan;
+  const int head = blockIdx.y;
+  for (int b = blockIdx.x; b < plan[PH_NSPLIT] * GR; b += gridDim.x) {
+    const PkvSplit t = ((const PkvSplit*)(plan + plan[PH_SPLIT]))[b / GR];
+    const int my = (b % GR) * 8 + (threadIdx.x >> 5), d = 4 * (threadIdx.x & 31);
+    const int pos = my / REP, r = my % REP;
+    if (pos >= min(t.n, a.rows - t.row)) continue;
+    auto unit = [&](int i) { return ((size_t)(t.first + i) * a.nkv + head) * TR + my; };
+    float M = -INFINITY;
+    for (int i = 0; i < t.parts; ++i) M = fmaxf(M, a.pre_ml[2 * unit(i)]);
+    const float R = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < t.parts; ++i) {
+      const size_t u = unit(i);
+      const float f = __builtin_amdgcn_exp2f(a.pre_ml[2 * u] - R);
+      L += f * a.pre_ml[2 * u + 1];
+      const f32x4 y = *(const f32x4*)(a.pre_o + u * HD + d);
+      // an item that a row sees nothing of has l = 0 and o = 0
+      x += y * f;
+    }
+    x *= 1.f / L;
+    const size_t at = ((size_t)(t.row + pos) * a.nkv * REP + head * REP + r) * HD + d;
+    if constexpr (A == ACT_F32) {
+      *(f32x4*)((float*)a.out + at) = x;
+    } else {
+      uint32_t* p = (uint32_t*)((uint16_t*)a.out + at);
+      p[0] = pack2<A == ACT_F16>(x[0], x[1]);
+      p[1] = pack2<A == ACT_F16>(x[2], x[3]);
+    }
+  }
+}
+
+template <int A, int REP>
+hipError_t launch_rep(const PkvAttnArgs& a, hipStream_t s) {
+  if (a.ndec > 0) {
+    hipLaunchKernelGGL((pkv_decode_kernel<A, REP>), dim3(a.ndec, a.nkv), dim3(64 * kDecWaves), 0, s, a);
+    if (a.ndec > a.ndseq || a.captured)
+      hipLaunchKernelGGL((pkv_decode_join_kernel<A, REP>), dim3(a.ndseq, a.nkv), dim3(REP * HD), 0, s, a);
+  }
+  if (a.npre > 0) {
+    hipLaunchKernelGGL((pkv_prefill_kernel<A, REP>), dim3(a.npre * a.nkv),
+                       dim3(64 * PreShape<A, REP>::NW), 0, s, a);
+    if (a.nsplit > 0 || a.captured)
+      hipLaunchKernelGGL((pkv_prefill_join_kernel<A, REP>),
+                         dim3(std::max(a.nsplit, 1) * (PreShape<A, REP>::TP * REP / 8), a.nkv), dim3(256),
+                         0, s, a);
+  }
+  return hipGetLastError();
+}
+template <int A>
+hipError_t launch_act(const PkvAttnArgs& a, hipStream_t s) {
+  switch (a.rep) {
+    case 1: return launch_rep<A, 1>(a, s);
+    case 2: return launch_rep<A, 2>(a, s);
+    case 4: return launch_rep<A, 4>(a, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace
+
+hipError_t launch_pkv_attn(int act, const PkvAttnArgs& a, hipStream_t s) {
+  if (act == ACT_F32) return launch_act<ACT_F32>(a, s);
+  if (act == ACT_F16) return launch_act<ACT_F16>(a, s);
+  return launch_act<ACT_BF16>(a, s);
+}
+
+int pkv_tile_positions(int act, int rep) {
+  auto of = [&](auto tag) {
+    constexpr int A = decltype(tag)::value;
+    return rep == 1 ? PreShape<A, 1>::TP : rep == 2 ? PreShape<A, 2>::TP : PreShape<A, 4>::TP;
+  };
+  return act == ACT_F32 ? of(std::integral_constant<int, ACT_F32>())
+                        : of(std::integral_constant<int, ACT_BF16>());
+}

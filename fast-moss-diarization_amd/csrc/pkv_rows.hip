@@ -1,0 +1,302 @@
+// Rows into and out of the paged 4-bit KV cache, and page copies.
+//
+// Append (Attention::forward's q/k norm, RoPE and cache append,
+// qwen3.rs:213-241, into 4-bit pages): with x a head's 128 values, g the gain,
+//   y = x / sqrt(mean(x^2) + eps) * g
+//   z[i] = y[i] cos[i] - y[i + 64] sin[i],  z[i + 64] = y[i + 64] cos[i] + y[i] sin[i]
+// q is z rounded once to the activation dtype; K is z and V the projection as
+// 32-bit values, held as blocks of 32 dims b: 2^e c[d], e the smallest integer
+// with max|b| <= 7 * 2^e and c the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 (ties
+// to the even code).  7 keeps every error within half a step of the widest
+// gap (6 would spend a bit of scale on maxima in (6, 7], 8 clips them by up to
+// a quarter); relative rms error of N(0, 1) blocks at 6 | 6.5 | 7 | 7.5 | 8:
+// .1155 | .1131 | .1119 | .1120 | .1151.
+//
+// K is computed in 64 bits (as fast as unpacked 32 bits on this device) and
+// rounded to 32: which code a value next to a border gets then does not depend
+// on the order of the mean's sum.  The wave's q heads take 32 bits.
+//
+// A token whose K or V of a head holds an infinity or a NaN gets scale 255 in
+// all eight blocks of that head: it reads back as NaN, and so does every
+// context that sees it.
+#include "fmd_common.h"
+#include "fmd_kernels.h"
+
+namespace {
+
+constexpr int HD = 128;
+
+// Lowest and highest block exponent: what a cache returns is a value of the
+// activation dtype (f16: 0.5 * 2^-23 is its smallest subnormal, 6 * 2^13 below
+// its largest value; 32-bit and bf16 caches end where sums over a cache of
+// 65,536 tokens still stay far inside 32 bits).
+template <int A> constexpr int kLo = A == ACT_F16 ? -23 : -64;
+template <int A> constexpr int kHi = A == ACT_F16 ? 13 : 64;
+
+// The sequence that holds `row`: the last one whose first row is <= row (one
+// with rows: a sequence without any starts where the next one does).
+__device__ __forceinline__ int seq_of(const int32_t* row0, int n, int row) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (row0[mid] <= row) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint8_t* pool_of(const int32_t* plan) {
+  return (uint8_t*)(((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL]);
+}
+
+// Head `h` of the page holding position `pos` of planned sequence `s`.
+__device__ __forceinline__ uint8_t* head_of(const int32_t* plan, int s, int pos, int layer, int nkv,
+                                            int h) {
+  const int page = plan[plan[plan[PH_TOFF] + s] + pos / kPkvPage];
+  return pool_of(plan) +
+         (((size_t)layer * plan[PH_PAGES] + page) * nkv + h) * (size_t)kPkvHeadBytes;
+}
+
+__device__ __forceinline__ int kscale_at(int t, int blk) {
+  return 64 * blk + 4 * (4 * (t >> 4) + (t & 3)) + ((t >> 2) & 3);
+}
+
+template <int A>
+__device__ __forceinline__ void load8(const void* p, size_t at, float* o) {
+  if constexpr (A == ACT_F32) {
+    const f32x4 a = *(const f32x4*)((const float*)p + at), b = *(const f32x4*)((const float*)p + at + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[i] = a[i];
+      o[4 + i] = b[i];
+    }
+  } else {
+    unpack8<A>(*(const u32x4*)((const uint16_t*)p + at), o);
+  }
+}
+template <int A>
+__device__ __forceinline__ void store8(void* p, size_t at, const float* v) {
+  if constexpr (A == ACT_F32) {
+    *(f32x4*)((float*)p + at) = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4*)((float*)p + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (uint32_t)st_act<A>(v[2 * i]) | ((uint32_t)st_act<A>(v[2 * i + 1]) << 16);
+    *(u32x4*)((uint16_t*)p + at) = w;
+  }
+}
+
+// Largest magnitude of the 32 dims that a quad of lanes holds, as bits
+// (magnitudes order like their bits, NaN above infinity).
+__device__ __forceinline__ uint32_t quad_max_bits(const float* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu);
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));
+  m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));
+  return m;
+}
+// Scale byte of a block whose largest magnitude has bits m: the float exponent
+// of m / 4, one more when the mantissa is above 1.75.
+template <int A>
+__device__ __forceinline__ int scale_byte(uint32_t m) {
+  const int e = (int)((m + 0x1fffffu) >> 23) - 2;
+  return min(max(e, 127 + kLo<A>), 127 + kHi<A>);
+}
+// Eight codes: v_cvt_scalef32_pk_fp4_f32 divides by the scale's power of two,
+// rounds to nearest even and saturates at 6.
+__device__ __forceinline__ uint32_t codes8(const float* x, int byte) {
+  const float sc = __builtin_bit_cast(float, (uint32_t)byte << 23);
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], sc, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], sc, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], sc, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], sc, 3);
+  return w;
+}
+
+// K (k) and V (v) of one token and head, 8 dims per lane of a 16-lane row.
+template <int A>
+__device__ __forceinline__ void store_kv(uint8_t* head, int t, int dc, const float* k, const float* v) {
+  const uint32_t mk = quad_max_bits(k), mv = quad_max_bits(v);
+  // any block of the row not finite: __ballot, then this row's 16 bits
+  const uint64_t bad = __ballot(mk >= 0x7f800000u || mv >= 0x7f800000u);
+  const bool nan = (bad >> (threadIdx.x & 48)) & 0xffffu;
+  const int bk = scale_byte<A>(mk), bv = scale_byte<A>(mv);
+  *(uint32_t*)(head + t * 64 + dc * 4) = nan ? 0u : codes8(k, bk);
+  *(uint32_t*)(head + kPkvV + t * 64 + dc * 4) = nan ? 0u : codes8(v, bv);
+  if ((dc & 3) == 0) {
+    head[kPkvKs + kscale_at(t, dc >> 2)] = (uint8_t)(nan ? 255 : bk);
+    head[kPkvVs + 64 * (dc >> 2) + t] = (uint8_t)(nan ? 255 : bv);
+  }
+}
+
+__device__ __forceinline__ double row16_sum(double v) {
+  // lanes ^1, ^2, ^7 and ^15 of the 16-lane row, as the 32-bit sum takes them
+#pragma unroll
+  for (int m : {1, 2, 7, 15}) v += __shfl_xor(v, m);
+  return v;
+}
+
+// Norm and rotation of the 8 dims 8 dc .. of a head, in F.
+template <class F>
+__device__ __forceinline__ void norm_rope(const float* x, const float* g, const float* c,
+                                          const float* s, int dc, float eps, float* z) {
+  F ss = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss += (F)x[i] * (F)x[i];
+  ss = row16_sum(ss);
+  const F r = (F)1 / sqrt(ss / (F)HD + (F)eps);
+  F y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (F)x[i] * r * (F)g[i];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const F o = __shfl_xor(y[i], 8);   // dim +- 64
+    z[i] = (float)(dc < 8 ? y[i] * (F)c[i] - o * (F)s[i] : y[i] * (F)c[i] + o * (F)s[i]);
+  }
+}
+
+// One work-group per row, 16 lanes per head: nh q heads, then nkv lane rows
+// that each take a head's K and V.
+template <int A>
+__global__ void pkv_append_kernel(PkvRowArgs a) {
+  const int32_t* plan = a.plan;
+  const int row = blockIdx.x;
+  if (row >= min(plan[PH_ROWS], a.rows)) return;
+  const int u = threadIdx.x >> 4, dc = threadIdx.x & 15;
+  if (u >= a.nh + a.nkv) return;     // whole 16-lane rows: the shuffles below stay inside one
+  const int s = seq_of(plan + plan[PH_ROW0], plan[PH_NSEQ], row);
+  const int pos = plan[plan[PH_POS0] + s] + row - plan[plan[PH_ROW0] + s];
+  const size_t base = (size_t)row * (a.nh + 2 * a.nkv) * HD + 8 * dc;
+  float x[8], g[8], c[8], sn[8], z[8];
+  load8<A>(a.x, base + (size_t)u * HD, x);
+  load8<A>(a.cos, (size_t)pos * (HD / 2) + 8 * (dc & 7), c);
+  load8<A>(a.sin, (size_t)pos * (HD / 2) + 8 * (dc & 7), sn);
+  if (u < a.nh) {
+    load8<A>(a.qn_w, 8 * dc, g);
+    norm_rope<float>(x, g, c, sn, dc, a.eps, z);
+    store8<A>(a.q_out, ((size_t)row * a.nh + u) * HD + 8 * dc, z);
+  } else {
+    float v[8];
+    load8<A>(a.x, base + (size_t)(u + a.nkv) * HD, v);
+    load8<A>(a.kn_w, 8 * dc, g);
+    norm_rope<double>(x, g, c, sn, dc, a.eps, z);
+    store_kv<A>(head_of(plan, s, pos, a.layer, a.nkv, u - a.nh), pos % kPkvPage, dc, z, v);
+  }
+}
+
+// K and V rows as they are (already rotated) into the plan's positions.
+template <int A>
+__global__ void pkv_write_kernel(PkvRowArgs a) {
+  const int32_t* plan = a.plan;
+  const int row = blockIdx.x;
+  if (row >= min(plan[PH_ROWS], a.rows)) return;
+  const int u = threadIdx.x >> 4, dc = threadIdx.x & 15;
+  if (u >= a.nkv) return;
+  const int s = seq_of(plan + plan[PH_ROW0], plan[PH_NSEQ], row);
+  const int pos = plan[plan[PH_POS0] + s] + row - plan[plan[PH_ROW0] + s];
+  const size_t at = ((size_t)row * a.nkv + u) * HD + 8 * dc;
+  float k[8], v[8];
+  load8<A>(a.x, at, k);
+  load8<A>(a.v, at, v);
+  store_kv<A>(head_of(plan, s, pos, a.layer, a.nkv, u), pos % kPkvPage, dc, k, v);
+}
+
+__device__ __forceinline__ void decode8(uint32_t w, int byte, float* o) {
+  const float sc = __builtin_bit_cast(float, (uint32_t)byte << 23);   // 255: every value NaN
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 0);
+  const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 1);
+  const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 2);
+  const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 3);
+  o[0] = a[0]; o[1] = a[1]; o[2] = b[0]; o[3] = b[1];
+  o[4] = c[0]; o[5] = c[1]; o[6] = d[0]; o[7] = d[1];
+}
+
+// The plan's rows back, as the values they stand for.
+template <int A>
+__global__ void pkv_read_kernel(PkvRowArgs a) {
+  const int32_t* plan = a.plan;
+  const int row = blockIdx.x;
+  if (row >= min(plan[PH_ROWS], a.rows)) return;
+  const int u = threadIdx.x >> 4, dc = threadIdx.x & 15;
+  if (u >= a.nkv) return;
+  const int s = seq_of(plan + plan[PH_ROW0], plan[PH_NSEQ], row);
+  const int pos = plan[plan[PH_POS0] + s] + row - plan[plan[PH_ROW0] + s];
+  const int t = pos % kPkvPage;
+  const uint8_t* head = head_of(plan, s, pos, a.layer, a.nkv, u);
+  float k[8], v[8];
+  decode8(*(const uint32_t*)(head + t * 64 + dc * 4), head[kPkvKs + kscale_at(t, dc >> 2)], k);
+  decode8(*(const uint32_t*)(head + kPkvV + t * 64 + dc * 4), head[kPkvVs + 64 * (dc >> 2) + t], v);
+  const size_t at = ((size_t)row * a.nkv + u) * HD + 8 * dc;
+  if (a.k_out) store8<A>(a.k_out, at, k);
+  if (a.v_out) store8<A>(a.v_out, at, v);
+}
+
+constexpr int kCopyUnroll = 4;
+
+// A page of a layer is contiguous: pairs x layers pieces of nkv * 544 16-byte
+// words, all of them one index range.
+__global__ void __launch_bounds__(256) pkv_copy_kernel(PkvPairs p, int n, uint32_t layers,
+                                                       uint32_t words, const u32x4* src, int src_pages, u32x4* dst,
+                                                       int dst_pages) {
+  const uint32_t total = (uint32_t)n * layers * words;   // below 2^31 (launch_pkv_copy)
+  const uint32_t at = blockIdx.x * (kCopyUnroll * 256) + threadIdx.x;
+  u32x4 w[kCopyUnroll];
+  size_t to[kCopyUnroll];
+#pragma unroll
+  for (int i = 0; i < kCopyUnroll; ++i) {
+    const uint32_t id = at + i * 256;
+    if (id >= total) continue;
+    const uint32_t piece = id / words, off = id - piece * words;
+    const uint32_t pair = piece / layers, layer = piece - pair * layers;
+    w[i] = src[((size_t)layer * src_pages + p.src[pair]) * words + off];
+    to[i] = ((size_t)layer * dst_pages + p.dst[pair]) * words + off;
+  }
+#pragma unroll
+  for (int i = 0; i < kCopyUnroll; ++i)
+    if (at + i * 256 < total) dst[to[i]] = w[i];
+}
+
+__global__ void pkv_clear_plan_kernel(int32_t* plan) {
+  if (threadIdx.x < PH_WORDS) plan[threadIdx.x] = 0;
+}
+
+}  // namespace
+
+#define BY_ACT(KERNEL, THREADS)                                                                    \
+  do {                                                                                             \
+    const dim3 grid(a.rows), block((THREADS + 63) / 64 * 64);                                      \
+    if (act == ACT_F32) hipLaunchKernelGGL(KERNEL<ACT_F32>, grid, block, 0, s, a);                 \
+    else if (act == ACT_F16) hipLaunchKernelGGL(KERNEL<ACT_F16>, grid, block, 0, s, a);            \
+    else hipLaunchKernelGGL(KERNEL<ACT_BF16>, grid, block, 0, s, a);                               \
+    return hipGetLastError();                                                                      \
+  } while (0)
+
+hipError_t launch_pkv_append(int act, const PkvRowArgs& a, hipStream_t s) {
+  BY_ACT(pkv_append_kernel, 16 * (a.nh + a.nkv));
+}
+hipError_t launch_pkv_write(int act, const PkvRowArgs& a, hipStream_t s) {
+  BY_ACT(pkv_write_kernel, 16 * a.nkv);
+}
+hipError_t launch_pkv_read(int act, const PkvRowArgs& a, hipStream_t s) {
+  BY_ACT(pkv_read_kernel, 16 * a.nkv);
+}
+
+hipError_t launch_pkv_copy(const PkvPairs& p, int n, int layers, int nkv, const void* src_pool,
+                           int src_pages, void* dst_pool, int dst_pages, hipStream_t s) {
+  const int words = nkv * (kPkvHeadBytes / 16);
+  const int64_t per = 256 * kCopyUnroll, groups = ((int64_t)n * layers * words + per - 1) / per;
+  if (n < 1 || n > kPkvPairs || (int64_t)n * layers * words > INT32_MAX - 2 * per) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(pkv_copy_kernel, dim3((unsigned)groups), dim3(256), 0, s, p, n, layers, words,
+                     (const u32x4*)src_pool, src_pages, (u32x4*)dst_pool, dst_pages);
+  return hipGetLastError();
+}
+
+hipError_t launch_pkv_clear_plan(int32_t* plan, hipStream_t s) {
+  hipLaunchKernelGGL(pkv_clear_plan_kernel, dim3(1), dim3(64), 0, s, plan);
+  return hipGetLastError();
+}

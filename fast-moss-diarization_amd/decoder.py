@@ -86,6 +86,7 @@ _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _U64 = ctypes.c_uint64
 _U32 = ctypes.c_uint32
+_I32 = ctypes.c_int32
 _SZ = ctypes.c_size_t
 
 # name -> (restype, argtypes); these are exactly the entry points of include/fmd_dec.h
@@ -128,6 +129,28 @@ SIGNATURES = {
     "fmd_op_attention_decode_noalloc": (_I, [_P, _P, _I, _P, _P, _I, _P]),
     "fmd_op_layer_decode": (_I, [_P, _P, _I, _P, _P, _I]),
     "fmd_op_logits": (_I, [_P, _P, _I, _P]),
+    "fmd_pkv_create": (_I, [_P, _I, _I, _I, _I, _I, ctypes.POINTER(_P)]),
+    "fmd_pkv_destroy": (_I, [_P]),
+    "fmd_pkv_bytes": (_SZ, [_P, _I]),
+    "fmd_pkv_open": (_I, [_P, ctypes.POINTER(_I32)]),
+    "fmd_pkv_fork": (_I, [_P, _I, ctypes.POINTER(_I32)]),
+    "fmd_pkv_copy": (_I, [_P, _I, ctypes.POINTER(_I32)]),
+    "fmd_pkv_free": (_I, [_P, _I]),
+    "fmd_pkv_truncate": (_I, [_P, _I, _I]),
+    "fmd_pkv_resize": (_I, [_P, _I]),
+    "fmd_pkv_len": (_I, [_P, _I]),
+    "fmd_pkv_free_pages": (_I, [_P]),
+    "fmd_pkv_pages": (_I, [_P, _I, _P, _I, ctypes.POINTER(_I32)]),
+    "fmd_pkv_pool": (_I, [_P, ctypes.POINTER(_P), ctypes.POINTER(_SZ)]),
+    "fmd_pkv_plan": (_I, [_P, _I, _P, _P]),
+    "fmd_op_pkv_append": (_I, [_P, _P, _I, _P, _P]),
+    "fmd_op_pkv_write": (_I, [_P, _P, _I, _P, _P]),
+    "fmd_op_pkv_read": (_I, [_P, _P, _I, _P, _P]),
+    "fmd_op_pkv_attention": (_I, [_P, _P, _I, _P, _P]),
+    "fmd_op_pkv_copy_pages": (_I, [_P, _I, _P, _P]),
+    "fmd_dec_step": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _P]),
+    "fmd_op_logprobs": (_I, [_P, _P, _I, _I, _I, _I64, _P, _I, _P, _P, _P, _P]),
+    "fmd_dec_logprobs": (_I, [_P, _I, _P, _I, _P, _P, _P, _P]),
     "fmd_enc_create": (_I, [ctypes.POINTER(FmdAudioConfig), _I, _I, ctypes.POINTER(_P)]),
     "fmd_enc_destroy": (_I, [_P]),
     "fmd_enc_set_stream": (_I, [_P, _P]),
@@ -263,6 +286,18 @@ class FinishReason(enum.IntEnum):
 class Generated:
     tokens: list[int]
     finish_reason: FinishReason
+
+
+@dataclass
+class TokenScores:
+    """Per row: log probability of the asked token (None without tokens), the
+    distribution's entropy (nats), the best alternatives and their log
+    probabilities, best first."""
+
+    logp: np.ndarray | None
+    entropy: np.ndarray
+    top_ids: np.ndarray
+    top_logp: np.ndarray
 
 
 class KvCache:
@@ -589,6 +624,32 @@ class Qwen3:
         _check(lib().fmd_dec_greedy(self.handle, batch, eos, _ptr(force), step, _ptr(done),
                                     _ptr(nxt), _ptr(emitted)))
         return nxt.tolist(), [int(v) if v != 0xFFFFFFFF else -1 for v in emitted]
+
+    # -- token scores ---------------------------------------------------------
+    def logprobs(self, batch: int, tokens: Sequence[int] | None = None, top: int = 0) -> "TokenScores":
+        """Scores of the logits that the last prefill, decode_step or step (of
+        `batch` rows) left on the device."""
+        tok = None if tokens is None else np.ascontiguousarray(np.asarray(tokens, dtype=np.uint32).reshape(-1))
+        if tok is not None and tok.size != batch:
+            raise FmdError(-1, "one token per row")
+        n, t = max(int(batch), 0), max(int(top), 0)
+        logp = None if tok is None else np.empty(n, dtype=np.float32)
+        s = TokenScores(logp, np.empty(n, dtype=np.float32), np.empty((n, t), dtype=np.uint32),
+                        np.empty((n, t), dtype=np.float32))
+        _check(lib().fmd_dec_logprobs(self.handle, batch, _ptr(tok), top, _ptr(logp), _ptr(s.entropy),
+                                      _ptr(s.top_ids), _ptr(s.top_logp)))
+        return s
+
+    def op_logprobs(self, logits_ptr: int, dtype: str, rows: int, vocab: int, targets_ptr: int | None,
+                    top: int, logp_ptr: int | None, entropy_ptr: int | None, ids_ptr: int | None,
+                    best_ptr: int | None, ld: int | None = None) -> None:
+        """Log probabilities of the int32 targets, entropies and the `top` best
+        alternatives of device logits (rows, vocab) in dtype "f32", "f16" or
+        "bf16", row stride ld (default vocab), into device buffers."""
+        code = {"f32": 0, "f16": 1, "bf16": 2}[dtype]
+        _check(lib().fmd_op_logprobs(self.handle, logits_ptr, code, rows, vocab,
+                                     vocab if ld is None else ld, targets_ptr, top, logp_ptr,
+                                     entropy_ptr, ids_ptr, best_ptr))
 
     # -- device ops (tests / benchmarks) -------------------------------------
     def set_stream(self, stream_handle: int | None) -> None:

@@ -60,6 +60,7 @@ typedef struct fmd_text_config {
 
 typedef struct fmd_dec fmd_dec;
 typedef struct fmd_kv fmd_kv;
+typedef struct fmd_pkv fmd_pkv;
 
 const char* fmd_last_error(void);
 
@@ -300,6 +301,116 @@ int fmd_op_attention_decode_noalloc(fmd_dec* dec, fmd_kv* kv, int layer, const v
  * to the device buffer logits_dev, rounded to the activation dtype first as
  * Qwen3::logits does. */
 int fmd_op_logits(fmd_dec* dec, const void* x_dev, int rows, float* logits_dev);
+
+/* --- paged KV cache in 4 bits ----------------------------------------------
+ *
+ * No counterpart in the reference, whose KvCache is one 16-bit block per
+ * micro-batch.  A pool of pages, each FMD_PKV_PAGE tokens of every layer, is
+ * shared by sequences that come, grow, fork and go on their own.  K (after the
+ * q/k norm and the rotation) and V are held as blocks of 32 dims of one token
+ * and head: 4-bit values 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign (e2m1), times
+ * 2^e in a scale byte, e the smallest with max|x| <= 7 * 2^e within [-23, 13]
+ * (f16 activations) or [-64, 64]; x / 2^e is rounded to the nearest value, ties
+ * to the even code, at most 6.  That is 4.25 bits a value, 136 bytes for a
+ * token's K and V of one head and layer.  A token whose K or V of a head holds
+ * an infinity or a NaN reads back as NaN in that head, as do the contexts that
+ * see it.
+ *
+ * Attention is causal.  With window > 0 a query at position p sees the keys
+ * j <= p with j > p - window or j < sinks; pages that no later query can see
+ * are given back by the next plan.
+ *
+ * A plan names sequences and how many new tokens each gets; the fmd_op_pkv_*
+ * calls then work on the plan's rows, sequence after sequence, tokens in
+ * order.  Rows of the callers' buffers behind the plan's are left as they are.
+ * Calls that change which pages belong to whom (fork, free, truncate, resize)
+ * end the plan.  Destroy a cache before its decoder.  Like a decoder, a cache
+ * is not re-entrant.
+ *
+ * The fmd_op_pkv_* calls with device buffers allocate nothing and can be
+ * captured into a graph: a replay works on the plan that is current when it
+ * runs, over at most as many rows, decode rows and many-token tiles as the
+ * captured call had (and finds no rows when there is no plan), so a graph that
+ * captured one new token for each sequence serves every later such plan.  All
+ * other fmd_pkv_* calls that touch pages are refused under capture.  Replays of
+ * graphs of one cache share its workspace: run them one after another. */
+#define FMD_PKV_PAGE 64
+
+/* `pages` pages (fmd_pkv_bytes), at most max_seqs sequences, at most max_rows
+ * new tokens in a plan.  Workspaces are allocated here, once. */
+int fmd_pkv_create(fmd_dec* dec, int pages, int max_seqs, int max_rows, int window, int sinks,
+                   fmd_pkv** out);
+int fmd_pkv_destroy(fmd_pkv* cache);
+size_t fmd_pkv_bytes(const fmd_dec* dec, int pages);
+/* A new, empty sequence; its number in *seq. */
+int fmd_pkv_open(fmd_pkv* cache, int32_t* seq);
+/* A new sequence with the same tokens.  fork shares the pages (a shared page is
+ * copied when one of its holders writes to it); copy copies them now. */
+int fmd_pkv_fork(fmd_pkv* cache, int seq, int32_t* out);
+int fmd_pkv_copy(fmd_pkv* cache, int seq, int32_t* out);
+/* Gives a sequence's number and pages back. */
+int fmd_pkv_free(fmd_pkv* cache, int seq);
+/* Keeps the first len tokens.  FMD_ERR_STATE when the window of a query at
+ * position len needs a page that was given back. */
+int fmd_pkv_truncate(fmd_pkv* cache, int seq, int len);
+/* Compacts the pages in use to the front of a pool of `pages` pages (the present
+ * number: in place, else a new pool, both in memory while it runs). */
+int fmd_pkv_resize(fmd_pkv* cache, int pages);
+int fmd_pkv_len(const fmd_pkv* cache, int seq);
+int fmd_pkv_free_pages(const fmd_pkv* cache);
+/* The sequence's page ids (-1: given back), at most `room` of them; *n: how
+ * many there are. */
+int fmd_pkv_pages(const fmd_pkv* cache, int seq, int32_t* out, int room, int32_t* n);
+/* The pool on the device, (layers, pages, kv_heads, 8704) bytes; moves with
+ * fmd_pkv_resize. */
+int fmd_pkv_pool(const fmd_pkv* cache, void** data, size_t* bytes);
+/* counts[i] new tokens for sequence seqs[i] (n different ones; 0 is allowed):
+ * pages are taken, shared ones copied, lengths grow.  FMD_ERR_OVERFLOW, with
+ * nothing changed, when the pages do not suffice. */
+int fmd_pkv_plan(fmd_pkv* cache, int n, const int32_t* seqs, const int32_t* counts);
+/* q/k norm and rotation of the raw fused projection qkv_dev (rows, q_dim + 2
+ * kv_dim), computed without rounding in between (K in 64 bits): q_dev (rows,
+ * q_dim) in the activation dtype, K and V into the pages of `layer`.  All
+ * device buffers here are 16-byte aligned. */
+int fmd_op_pkv_append(fmd_dec* dec, fmd_pkv* cache, int layer, const void* qkv_dev, void* q_dev);
+/* K (already rotated) and V, (rows, kv_heads, head_dim) activation-dtype rows,
+ * into the pages; and the plan's rows back out of them (either may be NULL). */
+int fmd_op_pkv_write(fmd_dec* dec, fmd_pkv* cache, int layer, const void* k_dev, const void* v_dev);
+int fmd_op_pkv_read(fmd_dec* dec, fmd_pkv* cache, int layer, void* k_dev, void* v_dev);
+/* Attention of the plan's rows over the pages of `layer`, which hold their own
+ * K and V too: q_dev, ctx_dev (rows, q_dim). */
+int fmd_op_pkv_attention(fmd_dec* dec, fmd_pkv* cache, int layer, const void* q_dev, void* ctx_dev);
+/* Copies page src[i] to page dst[i] in every layer (destinations different and
+ * none of them a source), whatever sequences they belong to. */
+int fmd_op_pkv_copy_pages(fmd_pkv* cache, int n, const int32_t* src, const int32_t* dst);
+/* The whole decoder over new tokens of n sequences (prompts, pieces of prompts
+ * and decode steps alike): a plan, then every layer, then the logits of each
+ * sequence's last new token (f32, (n, vocab), to `logits` on the host when
+ * non-NULL).  The tokens come as `ids` (host) or as `embeds`, (rows, hidden)
+ * activation-dtype rows (device when embeds_on_device).  When it fails, the
+ * sequences are as long as before. */
+int fmd_dec_step(fmd_dec* dec, fmd_pkv* cache, int n, const int32_t* seqs, const int32_t* counts,
+                 const uint32_t* ids, const void* embeds, int embeds_on_device, float* logits);
+
+/* --- token scores ----------------------------------------------------------
+ *
+ * No counterpart in the reference, which keeps the argmax alone.  Of each row x
+ * of logits: logp = x[target] - log sum exp x (NaN for an id outside the
+ * vocabulary), entropy = -sum p log p in nats, and the `top` (<= 32) best
+ * alternatives with their log probabilities, best first, equal logits by lower
+ * id, NaN below -inf.  -inf (a token that is ruled out) has probability 0; a
+ * row with a NaN or +inf, or -inf alone, has no distribution: NaN. */
+
+/* rows x vocab device logits in `dtype`, row stride ld; device targets (rows),
+ * logp (rows), entropy (rows), top_ids and top_logp (rows, top).  targets with
+ * logp, and entropy, may be NULL; top may be 0. */
+int fmd_op_logprobs(fmd_dec* dec, const void* logits_dev, fmd_dtype dtype, int rows, int vocab,
+                    int64_t ld, const int32_t* targets_dev, int top, float* logp_dev,
+                    float* entropy_dev, int32_t* top_ids_dev, float* top_logp_dev);
+/* The same of the logits of the last fmd_dec_prefill, fmd_dec_decode_step or
+ * fmd_dec_step (n rows), to host buffers (each may be NULL). */
+int fmd_dec_logprobs(fmd_dec* dec, int n, const uint32_t* tokens, int top, float* logp,
+                     float* entropy, uint32_t* top_ids, float* top_logp);
 
 /* --- audio path: Whisper encoder + VqAdaptor ------------------------------
  *
