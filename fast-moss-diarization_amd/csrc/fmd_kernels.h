@@ -311,8 +311,9 @@ struct PkvAttnArgs {
   void* out;             // (rows, nh, hd)
   int window, sinks;     // window 0: every key up to the query's own
   float scale;
-  int ndec, ndseq, npre, nsplit;   // the plan's counts when the call was made
+  int ndec, npre, nsplit;   // the plan's counts when the call was made
   int captured;          // into a graph, whose replays may need joins that this plan does not
+  uint32_t* tickets;     // (slots, nkv), 0 between launches
   float* dec_ml;         // (slots, nkv, rep, 2)
   float* dec_o;          // (slots, nkv, rep, hd)
   float* pre_ml;         // (slots, nkv, tile rows, 2)
@@ -336,5 +337,6 @@ struct LogprobArgs {
   void* work;            // logprob_work_bytes()
 };
 int logprob_max_top();
-size_t logprob_work_bytes();   // enough for every call
+size_t logprob_work_bytes();     // enough for every call
+size_t logprob_ticket_words();   // of it, the first words: 0 before the first call
 hipError_t launch_logprobs(const LogprobArgs& a, hipStream_t s);

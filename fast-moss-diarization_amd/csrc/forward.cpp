@@ -1308,6 +1308,7 @@ int logprob_args(fmd_dec* d, const void* x, int dtype, int rows, int vocab, int6
     if (cap != hipStreamCaptureStatusNone)
       return fmd_fail(FMD_ERR_STATE, "the first call of a handle allocates: make one before capturing");
     CHK(d->ws.lpwork.ensure(logprob_work_bytes()));
+    LAUNCH(launch_fill_i32(d->ws.lpwork.as<int32_t>(), (int64_t)logprob_ticket_words(), 0, d->stream));
   }
   LogprobArgs a{};
   a.x = x;

@@ -35,13 +35,13 @@ struct fmd_pkv {
   DevBuf pool;
   // the current plan
   bool planned = false;
-  int rows = 0, ndec = 0, ndseq = 0, npre = 0, nsplit = 0;
+  int rows = 0, ndec = 0, npre = 0, nsplit = 0;
   DevBuf plan;
   PkvBounds most{};
   int32_t* stage[2] = {nullptr, nullptr};   // pinned; a slot is rewritten once its upload has passed
   hipEvent_t staged[2] = {nullptr, nullptr};
   int slot = 0;
-  DevBuf dec_ml, dec_o, pre_ml, pre_o;      // partial results of rows in several items
+  DevBuf tickets, dec_ml, dec_o, pre_ml, pre_o;      // partial results of rows in several items
 };
 
 namespace {
@@ -164,12 +164,12 @@ int pkv_attention(fmd_pkv* c, int layer, const void* q, void* ctx) {
   a.sinks = c->tab.sinks;
   a.scale = d->scale;
   a.ndec = c->ndec;
-  a.ndseq = c->ndseq;
   a.npre = c->npre;
   a.nsplit = c->nsplit;
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   HIPCHK(hipStreamIsCapturing(d->stream, &cap));
   a.captured = cap != hipStreamCaptureStatusNone;
+  a.tickets = c->tickets.as<uint32_t>();
   a.dec_ml = c->dec_ml.as<float>();
   a.dec_o = c->dec_o.as<float>();
   a.pre_ml = c->pre_ml.as<float>();
@@ -189,7 +189,7 @@ extern "C" int fmd_pkv_destroy(fmd_pkv* c) {
   if (!c) return 0;
   hipSetDevice(c->dec->device);
   hipStreamSynchronize(c->dec->stream);
-  for (DevBuf* b : {&c->pool, &c->plan, &c->dec_ml, &c->dec_o, &c->pre_ml, &c->pre_o}) b->release();
+  for (DevBuf* b : {&c->pool, &c->plan, &c->tickets, &c->dec_ml, &c->dec_o, &c->pre_ml, &c->pre_o}) b->release();
   for (int i = 0; i < 2; ++i) {
     if (c->staged[i]) hipEventDestroy(c->staged[i]);
     if (c->stage[i]) hipHostFree(c->stage[i]);
@@ -225,6 +225,7 @@ extern "C" int fmd_pkv_create(fmd_dec* d, int pages, int max_seqs, int max_rows,
   const size_t pre_units = max_rows > 1 ? (size_t)c->most.pre_slots * d->nkv * tile * d->rep : 0;
   rc = c->pool.ensure(fmd_pkv_bytes(d, pages));
   if (!rc) rc = c->plan.ensure(c->most.words * 4);
+  if (!rc) rc = c->tickets.ensure((size_t)c->most.dec_items * d->nkv * 4);
   if (!rc) rc = c->dec_ml.ensure(dec_units * 8);
   if (!rc) rc = c->dec_o.ensure(dec_units * d->hd * 4);
   if (!rc) rc = c->pre_ml.ensure(pre_units * 8);
@@ -242,7 +243,9 @@ extern "C" int fmd_pkv_create(fmd_dec* d, int pages, int max_seqs, int max_rows,
       rc = fmd_fail(FMD_ERR_HIP, "event creation failed");
     }
   }
-  if (!rc && launch_pkv_clear_plan(c->plan.as<int32_t>(), d->stream) != hipSuccess)
+  if (!rc && (launch_pkv_clear_plan(c->plan.as<int32_t>(), d->stream) != hipSuccess ||
+              launch_fill_i32(c->tickets.as<int32_t>(), (int64_t)c->most.dec_items * d->nkv, 0, d->stream) !=
+                  hipSuccess))
     rc = fmd_fail(FMD_ERR_HIP, "plan clear failed");
   if (!rc && hipStreamSynchronize(d->stream) != hipSuccess) rc = fmd_fail(FMD_ERR_HIP, "sync failed");
   if (rc) {
@@ -381,7 +384,6 @@ extern "C" int fmd_pkv_plan(fmd_pkv* c, int n, const int32_t* seqs, const int32_
     c->slot ^= 1;
     c->rows = w[PH_ROWS];
     c->ndec = w[PH_NDEC];
-    c->ndseq = w[PH_NDSEQ];
     c->npre = w[PH_NPRE];
     c->nsplit = w[PH_NSPLIT];
     c->planned = true;

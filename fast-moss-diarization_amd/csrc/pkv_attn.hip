@@ -8,8 +8,8 @@
 // and the sums over v are 32 bits.
 //
 // One new token (a decode step) is bound by the cache's bytes, 136 per key and
-// KV head.  A wave takes whole pages: K codes go to registers, V codes by
-// direct-to-LDS copies, the next page's in flight while this one is computed.
+// KV head.  A wave takes whole pages, by direct-to-LDS copies, the next page's in
+// flight while this one is computed.
 // - S^T = K q^T by 16x16x32 MFMAs: lane (c, g) = (l % 16, l / 16) of tile mt
 //   holds row c of the A operand, which is token 16 (c/4) + 4 mt + c%4, and of
 //   it the dims of block g, whose scale is then one per lane:
@@ -24,8 +24,8 @@
 //   alone keeps 8 (32-bit activations: three terms, 24 bits).
 // - O^T += V^T P^T with V's codes transposed by LDS 4-bit transpose reads (lane
 //   = dim, 16 tokens in 8 bytes) and widened without a scale.
-// The units' pages are cut into items so that a launch fills the device; a
-// second kernel joins the items of a row.
+// A row's pages are cut into items so that a launch fills the device; the last
+// of a row's items to end joins them.
 //
 // Many new tokens (prefill) are bound by the products and the softmax.  A
 // work-group holds the queries of a tile, waves own (head, 16 QS positions);
@@ -107,22 +107,42 @@ __device__ __forceinline__ const uint8_t* pool_of(const int32_t* plan) {
   return (const uint8_t*)(((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL]);
 }
 
+// Words that one work-group leaves for another of the same launch.
+__device__ __forceinline__ void put(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // ---- one new token --------------------------------------------------------
 
 constexpr int kDecWaves = 4;
 
+// The plan, which no kernel that reads it here writes: scalar loads, whose
+// counter the waits for the copies below do not share.
+typedef const __attribute__((address_space(4))) int32_t* plan_t;
+__device__ __forceinline__ plan_t plan_of(const int32_t* p) { return (plan_t)(uint64_t)(uintptr_t)p; }
+
 template <int A, int REP>
-__global__ void __launch_bounds__(64 * kDecWaves) pkv_decode_kernel(PkvAttnArgs a) {
+__global__ void __launch_bounds__(64 * kDecWaves, 2) pkv_decode_kernel(PkvAttnArgs a) {
   constexpr bool F16 = A == ACT_F16;
   constexpr int NT = A == ACT_F32 ? 3 : 1;          // terms of q
   constexpr int PT = A == ACT_F32 ? 3 : 2;          // terms of p
   constexpr int TPP = 4 / REP;                      // terms that the columns of one MFMA hold
   constexpr int PASSES = (PT + TPP - 1) / TPP;
-  constexpr int VB = 4096;                          // V codes of a page and head
-  __shared__ __attribute__((aligned(1024))) uint8_t sV[kDecWaves][2][VB];
+  constexpr int ESZ = A == ACT_F32 ? 4 : 2;
+  constexpr int QB = REP * HD * ESZ;                // bytes of the group's queries
+  constexpr int QC = (QB + 1023) / 1024;            // copies of 1 KiB for them
+  constexpr int SLOT = kPkvHeadBytes;               // a page of one head
+  constexpr int COPIES = 9;                         // copies of 1 KiB (the last of 512 B) for it
+  // per wave: two pages and the queries, all by direct-to-LDS copies, so that the
+  // only loads that are waited for are counted here
+  __shared__ __attribute__((aligned(1024))) uint8_t sPage[kDecWaves][2 * SLOT + 1024 * QC];
   __shared__ float sM[kDecWaves][REP], sL[kDecWaves][REP];
-  float* const sO = (float*)&sV[0][0][0];           // [wave][REP][HD], after the loop
-  const int32_t* plan = a.plan;
+  __shared__ uint32_t sTicket;
+  float* const sO = (float*)&sPage[0][0];           // [wave][REP][HD], after the loop
+  const plan_t plan = plan_of(a.plan);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c = lane & 15, g = lane >> 4;
   const int head = blockIdx.y, nh = a.nkv * REP;
@@ -130,74 +150,95 @@ __global__ void __launch_bounds__(64 * kDecWaves) pkv_decode_kernel(PkvAttnArgs 
   const float c2 = a.scale * kLog2e;
   const int n_items = plan[PH_NDEC];
   const size_t stride = (size_t)a.nkv * kPkvHeadBytes;       // bytes of a page
-  const uint8_t* layer = pool_of(plan) + (size_t)a.layer * plan[PH_PAGES] * stride +
-                         (size_t)head * kPkvHeadBytes;
-  const uint32_t lv = lds_addr(sV[w]);
-  // V copy: instruction j brings tokens 16 j .. 16 j + 15; token t's 16-byte
-  // chunk x lies at chunk x ^ ((t / 4) % 4), so that a transpose read's 16
-  // tokens fall in distinct banks
-  uint32_t vsrc[4];
+  const uint8_t* layer =
+      (const uint8_t*)(((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL]) +
+      (size_t)a.layer * plan[PH_PAGES] * stride + (size_t)head * kPkvHeadBytes;
+  uint8_t* const mine = &sPage[w][0];
+  const uint32_t lds = lds_addr(mine);
+  // Copy j < 4 brings the K codes of tokens 16 j .. 16 j + 15, j + 4 their V
+  // codes.  Token t's 16-byte chunk x lies at chunk x ^ (t / 16) for K and x ^
+  // ((t / 4) % 4) for V: the 16 tokens of a fragment read, and those of a
+  // transpose read, then fall in distinct banks.
+  uint32_t ksrc[4], vsrc;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int t = 16 * j + (lane >> 2);
-    vsrc[j] = (uint32_t)(t * 64 + (((lane & 3) ^ ((t >> 2) & 3)) << 4));
-  }
-  const uint32_t ksrc = (uint32_t)((16 * (c >> 2) + (c & 3)) * 64 + 16 * g);   // + 256 mt
+  for (int j = 0; j < 4; ++j)
+    ksrc[j] = (uint32_t)((16 * j + (lane >> 2)) * 64 + (((lane & 3) ^ j) << 4));
+  vsrc = (uint32_t)(kPkvV + (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 4) & 3)) << 4));   // + 1024 j
+  auto fetch = [&](int id, int slot) {
+    const uint8_t* page = layer + (size_t)id * stride;
+    const uint32_t to = lds + slot * SLOT;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lds_copy16(page, ksrc[j], to + j * 1024);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) lds_copy16(page, vsrc + j * 1024, to + kPkvV + j * 1024);
+    if (lane < 32) lds_copy16(page, (uint32_t)(kPkvKs + 16 * lane), to + kPkvKs);
+  };
 
   for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
-    const PkvDecItem item = ((const PkvDecItem*)(plan + PH_WORDS))[it];
+    const plan_t ip = plan + PH_WORDS + it * (int)(sizeof(PkvDecItem) / 4);
+    PkvDecItem item;
+    item.row = ip[0];
+    item.pos = ip[1];
+    item.table = ip[2];
+    item.sp = ip[3];
+    item.wp = ip[4];
+    item.v0 = ip[5];
+    item.v1 = ip[6];
+    item.slot = ip[7];
+    item.first = ip[8];
+    item.parts = ip[9];
     if (item.row >= a.rows) continue;
-    const int32_t* table = plan + item.table;
+    const plan_t table = plan + item.table;
     auto page_of = [&](int v) { return v < item.sp ? v : item.wp + (v - item.sp); };
-    u32x4 qf[4][NT];
+    auto id_of = [&](int v) { return table[page_of(min(v, item.v1 - 1))]; };   // read a step ahead
+    const int first = item.v0 + w;
+    int id = id_of(first);
+    {
+      const uint8_t* q = (const uint8_t*)a.q + ((size_t)item.row * nh + head * REP) * (HD * ESZ);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      load_terms<A, NT>(a.q, ((size_t)item.row * nh + head * REP + c % REP) * HD + 32 * g + 8 * j, true,
-                        qf[j]);
+      for (int j = 0; j < QC; ++j)
+        if (j * 1024 + 16 * lane < QB) lds_copy16(q, (uint32_t)(j * 1024 + 16 * lane), lds + 2 * SLOT + j * 1024);
+    }
+    if (first < item.v1) fetch(id, 0);
+    id = id_of(first + kDecWaves);
     f32x4 o[8];
 #pragma unroll
     for (int d = 0; d < 8; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m2 = -INFINITY, mr = 0.f, l = 0.f;   // mr: m2, or 0 while no key was seen
+    u32x4 qf[4][NT];
 
-    u32x4 kn[4], vsn;
-    uint32_t ksn = 0;
-    // id: the page to fetch, read one step ahead of its use
-    auto id_of = [&](int v) { return v < item.v1 ? table[page_of(v)] : 0; };
-    auto fetch = [&](int id, int buf) {
-      const uint8_t* page = layer + (size_t)__builtin_amdgcn_readfirstlane(id) * stride;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        lds_copy16(page + kPkvV, vsrc[j], lv + buf * VB + j * 1024);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) kn[mt] = *(const u32x4*)(page + ksrc + 256 * mt);
-      ksn = *(const uint32_t*)(page + kPkvKs + 4 * (16 * g + c));
-      vsn = *(const u32x4*)(page + kPkvVs + 64 * blk + 16 * g);
-    };
-    int buf = 0, id = id_of(item.v0 + w + kDecWaves);
-    if (item.v0 + w < item.v1) fetch(id_of(item.v0 + w), 0);
-    for (int v = item.v0 + w; v < item.v1; v += kDecWaves, buf ^= 1) {
-      u32x4 k[4], vs = vsn;
-      const uint32_t ks = ksn;
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) k[mt] = kn[mt];
-      // this page's registers and V codes are there, and the reads of the buffer
-      // that the next page's go to are done
-      __builtin_amdgcn_s_waitcnt(0x70);   // vmcnt(0) lgkmcnt(0)
-      asm volatile("" ::: "memory");
+    int slot = 0;
+    for (int v = first; v < item.v1; v += kDecWaves, slot ^= 1) {
+      // the next page's copies go out, this page's are waited for.  The slot they
+      // go to was read in the step before: its reads have been answered, since
+      // what they brought has been used.
       if (v + kDecWaves < item.v1) {
-        fetch(id, buf ^ 1);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        fetch(id, slot ^ 1);
         id = id_of(v + 2 * kDecWaves);
+        wait_vm<COPIES>();
+      } else {
+        wait_vm<0>();
       }
-
+      asm volatile("" ::: "memory");
+      if (v == first) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          load_terms<A, NT>(mine + 2 * SLOT, (size_t)(c % REP) * HD + 32 * g + 8 * j, true, qf[j]);
+      }
+      const uint8_t* page = mine + slot * SLOT;
       const int kb = page_of(v) * kPkvPage;
+      const uint32_t ks = *(const uint32_t*)(page + kPkvKs + 4 * (16 * g + c));
+      const u32x4 vs = *(const u32x4*)(page + kPkvVs + 64 * blk + 16 * g);
       f32x4 s[4];
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         const float sc = __builtin_bit_cast(float, ((ks >> (8 * mt)) & 0xffu) << 23);
+        const u32x4 k = *(const u32x4*)(page + (16 * (c >> 2) + 4 * mt + (c & 3)) * 64 + ((g ^ (c >> 2)) << 4));
         s[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const u32x4 kf = widen8<F16>(k[mt][j], sc);
+          const u32x4 kf = widen8<F16>(k[j], sc);
 #pragma unroll
           for (int n = 0; n < NT; ++n) s[mt] = mfma<F16>(kf, qf[j][n], s[mt]);
         }
@@ -237,7 +278,7 @@ __global__ void __launch_bounds__(64 * kDecWaves) pkv_decode_kernel(PkvAttnArgs 
         const uint32_t byte = (vs[e >> 2] >> (8 * (e & 3))) & 0xffu;
         p[e] = __builtin_amdgcn_exp2f(x + ((float)byte - 127.f));
       }
-      const uint8_t* vb = &sV[w][buf][0];
+      const uint8_t* vb = page + kPkvV;
       typedef int i32x2 __attribute__((ext_vector_type(2)));
       typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
       u32x4 pf[PASSES][2];
@@ -275,6 +316,7 @@ __global__ void __launch_bounds__(64 * kDecWaves) pkv_decode_kernel(PkvAttnArgs 
         }
       }
     }
+    wait_vm<0>();   // the queries of a wave without pages, too
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
     // the terms of a column add up; dims 32 b .. come from block b's columns
@@ -297,8 +339,17 @@ __global__ void __launch_bounds__(64 * kDecWaves) pkv_decode_kernel(PkvAttnArgs 
       sL[w][c] = l;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < REP * HD; i += 64 * kDecWaves) {
-      const int r = i / HD, d = i % HD;
+    // (m, l, o) of the item's waves joined, REP * HD values over the threads
+    constexpr int NV = (REP * HD + 64 * kDecWaves - 1) / (64 * kDecWaves);
+    const bool whole = item.parts == 1;
+    auto value = [&](int k) { return (int)threadIdx.x + k * 64 * kDecWaves; };
+    auto store = [&](int i, float x, float L) {
+      ((typename ActT<A>::T*)a.out)[((size_t)item.row * nh + head * REP) * HD + i] = st_act<A>(x / L);
+    };
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int i = value(k), r = i / HD;
+      if (i >= REP * HD) break;
       float M = sM[0][r];
 #pragma unroll
       for (int j = 1; j < kDecWaves; ++j) M = fmaxf(M, sM[j][r]);
@@ -309,43 +360,67 @@ __global__ void __launch_bounds__(64 * kDecWaves) pkv_decode_kernel(PkvAttnArgs 
         // a wave without pages has m = -inf, l = 0 and o = 0
         const float f = __builtin_amdgcn_exp2f(sM[j][r] - R);
         L += f * sL[j][r];
-        x += f * sO[(j * REP + r) * HD + d];
+        x += f * sO[j * REP * HD + i];
       }
-      if (item.slot < 0) {
-        ((typename ActT<A>::T*)a.out)[((size_t)item.row * nh + head * REP + r) * HD + d] = st_act<A>(x / L);
+      if (whole) {
+        store(i, x, L);
       } else {
-        const size_t u = ((size_t)item.slot * a.nkv + head) * REP + r;
-        a.dec_o[u * HD + d] = x;
-        if (d == 0) {
-          a.dec_ml[2 * u] = M;
-          a.dec_ml[2 * u + 1] = L;
+        // past the XCD's own L2: the row's last item reads them
+        const size_t u = ((size_t)item.slot * a.nkv + head) * REP;
+        put(a.dec_o + u * HD + i, x);
+        if (i % HD == 0) {
+          put(a.dec_ml + 2 * (u + r), M);
+          put(a.dec_ml + 2 * (u + r) + 1, L);
+        }
+      }
+    }
+    if (!whole) {
+      // A ticket, drawn once this work-group's stores have been answered: the
+      // last of a row's items finds all of them and joins them.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      uint32_t* const ticket = a.tickets + (size_t)item.first * a.nkv + head;
+      if (threadIdx.x == 0) sTicket = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      if (sTicket == (uint32_t)item.parts - 1) {
+        if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int i = value(k), r = i / HD;
+          if (i >= REP * HD) break;
+          auto unit = [&](int p) { return ((size_t)(item.first + p) * a.nkv + head) * REP; };
+          // parts in blocks of eight, each with a running maximum: the loads of
+          // a block are in flight together
+          float M = -INFINITY, L = 0.f, x = 0.f;
+          for (int p0 = 0; p0 < item.parts; p0 += 8) {
+            float m8[8], l8[8], o8[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+              const size_t u = unit(min(p0 + p, item.parts - 1));
+              m8[p] = get(a.dec_ml + 2 * (u + r));
+              l8[p] = get(a.dec_ml + 2 * (u + r) + 1);
+              o8[p] = get(a.dec_o + u * HD + i);
+            }
+            float N = M;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) N = fmaxf(N, m8[p]);
+            const float R = N == -INFINITY ? 0.f : N, f0 = __builtin_amdgcn_exp2f(M - R);
+            L *= f0;
+            x *= f0;
+            M = N;
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+              if (p0 + p >= item.parts) break;
+              const float f = __builtin_amdgcn_exp2f(m8[p] - R);
+              L += f * l8[p];
+              x += f * o8[p];
+            }
+          }
+          store(i, x, L);
         }
       }
     }
     __syncthreads();   // before the next item's copies overwrite sO
-  }
-}
-
-// Joins the items of each row: one work-group per (sequence, KV head).
-template <int A, int REP>
-__global__ void __launch_bounds__(REP * HD) pkv_decode_join_kernel(PkvAttnArgs a) {
-  const int32_t* plan = a.plan;
-  const int head = blockIdx.y, r = threadIdx.x / HD, d = threadIdx.x % HD;
-  for (int s = blockIdx.x; s < plan[PH_NDSEQ]; s += gridDim.x) {
-    const PkvDecSeq q = ((const PkvDecSeq*)(plan + plan[PH_DSEQ]))[s];
-    if (q.n < 2 || q.row >= a.rows) continue;
-    auto unit = [&](int i) { return ((size_t)(q.first + i) * a.nkv + head) * REP + r; };
-    float M = -INFINITY;
-    for (int i = 0; i < q.n; ++i) M = fmaxf(M, a.dec_ml[2 * unit(i)]);
-    const float R = M == -INFINITY ? 0.f : M;
-    float L = 0.f, x = 0.f;
-    for (int i = 0; i < q.n; ++i) {
-      const size_t u = unit(i);
-      const float f = __builtin_amdgcn_exp2f(a.dec_ml[2 * u] - R);
-      L += f * a.dec_ml[2 * u + 1];
-      x += f * a.dec_o[u * HD + d];
-    }
-    ((typename ActT<A>::T*)a.out)[((size_t)q.row * a.nkv * REP + head * REP + r) * HD + d] = st_act<A>(x / L);
   }
 }
 
@@ -629,11 +704,8 @@ __global__ void __launch_bounds__(256) pkv_prefill_join_kernel(PkvAttnArgs a) {
 
 template <int A, int REP>
 hipError_t launch_rep(const PkvAttnArgs& a, hipStream_t s) {
-  if (a.ndec > 0) {
+  if (a.ndec > 0)
     hipLaunchKernelGGL((pkv_decode_kernel<A, REP>), dim3(a.ndec, a.nkv), dim3(64 * kDecWaves), 0, s, a);
-    if (a.ndec > a.ndseq || a.captured)
-      hipLaunchKernelGGL((pkv_decode_join_kernel<A, REP>), dim3(a.ndseq, a.nkv), dim3(REP * HD), 0, s, a);
-  }
   if (a.npre > 0) {
     hipLaunchKernelGGL((pkv_prefill_kernel<A, REP>), dim3(a.npre * a.nkv),
                        dim3(64 * PreShape<A, REP>::NW), 0, s, a);

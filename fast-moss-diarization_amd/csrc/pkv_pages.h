@@ -34,13 +34,11 @@ enum PkvHdr {
   PH_POOL = 2,     // pool address, low and high word
   PH_PAGES = 4,    // pages of the pool (the layer stride)
   PH_NDEC = 5,     // decode items, in front of the other sections
-  PH_NDSEQ = 6,    // sequences with one new token
   PH_NPRE = 7,     // many-token items
   PH_NSPLIT = 8,   // many-token tiles cut into several items
   PH_ROW0 = 9,     // offset: first row of each sequence, and the row count
   PH_POS0 = 10,    // offset: position of that row
   PH_TOFF = 11,    // offset: where the sequence's page ids are
-  PH_DSEQ = 12,    // offset: PkvDecSeq entries
   PH_PITEM = 13,   // offset: PkvPreItem entries
   PH_SPLIT = 14,   // offset: PkvSplit entries
   PH_WORDS = 32
@@ -48,10 +46,9 @@ enum PkvHdr {
 // The visible pages of an item's queries, in order: pages [0, sp) (the sinks),
 // then pages wp, wp + 1, ..; v counts through both.
 struct PkvDecItem {
-  int32_t row, pos, table, sp, wp, v0, v1, slot;   // slot < 0: the item is its row's only one
-};
-struct PkvDecSeq {
-  int32_t row, first, n, pad;                      // partial slots first .. first + n - 1
+  int32_t row, pos, table, sp, wp, v0, v1;
+  int32_t slot, first, parts;                      // its partial slot, of first .. first + parts - 1 of its row
+  int32_t pad[2];
 };
 struct PkvPreItem {
   int32_t row, pos, n, table, sp, wp, v0, v1, slot, pad[3];
@@ -300,7 +297,7 @@ class PkvPages {
 
 // Work-groups that the attention's items are cut for, over all KV heads, and
 // the pages of an item at least (a decode work-group's four waves take one each).
-constexpr int kPkvDecGroups = 1024, kPkvPreGroups = 512;
+constexpr int kPkvDecGroups = 512, kPkvPreGroups = 512;
 constexpr int kPkvDecMinPages = 4, kPkvPreMinPages = 8;
 
 // What a plan takes at most.  Decode: an item's pages are at least all rows'
@@ -317,7 +314,7 @@ inline PkvBounds pkv_bounds(int nkv, int max_seqs, int max_rows, int max_len, in
   b.dec_items = kPkvDecGroups / nkv + max_seqs + 1;
   b.tiles = max_rows / tile + max_seqs;
   b.pre_slots = 2 * (kPkvPreGroups / nkv + 1);
-  b.words = PH_WORDS + ((size_t)b.dec_items * sizeof(PkvDecItem) + (size_t)max_seqs * sizeof(PkvDecSeq) +
+  b.words = PH_WORDS + ((size_t)b.dec_items * sizeof(PkvDecItem) +
                         (size_t)(b.tiles + b.pre_slots) * sizeof(PkvPreItem) +
                         (size_t)b.pre_slots * sizeof(PkvSplit)) / 4 +
             3 * (size_t)max_seqs + 1 + (size_t)max_seqs * pkv_ceil(max_len, kPkvPage);
@@ -343,11 +340,22 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
     rows += counts[i];
   }
   std::vector<PkvDecItem> di;
-  std::vector<PkvDecSeq> ds;
   std::vector<PkvPreItem> pi;
   std::vector<PkvSplit> sp;
   std::vector<int32_t> toff(n, 0), table;
-  const int dec_per = std::max(kPkvDecMinPages, pkv_ceil(dec_pages * nkv, kPkvDecGroups));
+  // as many pages to an item as it takes for the items to fit the device's
+  // work-group slots in one round, if they can
+  int dec_per = std::max(kPkvDecMinPages, pkv_ceil(dec_pages * nkv, kPkvDecGroups));
+  auto dec_items = [&]() {
+    int64_t k = 0;
+    for (const Row& r : order)
+      if (r.n == 1) k += pkv_ceil(c.visible(r.pos, r.pos).n, dec_per);
+    return k;
+  };
+  int dec_rows = 0;
+  for (const Row& r : order) dec_rows += r.n == 1;
+  while ((int64_t)dec_rows * nkv <= kPkvDecGroups && dec_items() * nkv > kPkvDecGroups)
+    dec_per += std::max(1, dec_per / 16);
   const int pre_per = std::max(kPkvPreMinPages, pkv_ceil(pre_pages * nkv, kPkvPreGroups));
   int dec_slots = 0, pre_slots = 0;
   for (int i = 0; i < n; ++i) {
@@ -357,11 +365,10 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
     if (r.n == 1) {
       const PkvPages::Visible v = c.visible(r.pos, r.pos);
       const int per = pkv_ceil(v.n, pkv_ceil(v.n, dec_per)), parts = pkv_ceil(v.n, per);
-      ds.push_back({r.row, dec_slots, parts, 0});
       for (int k = 0; k < parts; ++k)
-        di.push_back({r.row, r.pos, i, v.sp, v.wp, k * per, std::min((k + 1) * per, v.n),
-                      parts > 1 ? dec_slots + k : -1});
-      dec_slots += parts > 1 ? parts : 0;
+        di.push_back({r.row, r.pos, i, v.sp, v.wp, k * per, std::min((k + 1) * per, v.n), dec_slots + k,
+                      dec_slots, parts, {0, 0}});
+      dec_slots += parts;
     } else {
       for (int p = 0; p < r.n; p += tile) {
         const int m = std::min(tile, r.n - p);
@@ -387,9 +394,9 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
     return at;
   };
   // the sections' sizes are known: the tables come last, behind `table_at`
-  const size_t di_words = di.size() * sizeof(PkvDecItem) / 4, ds_words = ds.size() * sizeof(PkvDecSeq) / 4,
+  const size_t di_words = di.size() * sizeof(PkvDecItem) / 4,
                pi_words = pi.size() * sizeof(PkvPreItem) / 4, sp_words = sp.size() * sizeof(PkvSplit) / 4;
-  const int table_at = (int)(PH_WORDS + di_words + 3 * (size_t)n + 1 + ds_words + pi_words + sp_words);
+  const int table_at = (int)(PH_WORDS + di_words + 3 * (size_t)n + 1 + pi_words + sp_words);
   for (PkvDecItem& x : di) x.table = table_at + toff[x.table];
   for (PkvPreItem& x : pi) x.table = table_at + toff[x.table];
   put(di.data(), di_words);
@@ -400,7 +407,6 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
     w[at_toff + i] = table_at + toff[i];
   }
   w[at_row0 + n] = rows;
-  w[PH_DSEQ] = put(ds.data(), ds_words);
   w[PH_PITEM] = put(pi.data(), pi_words);
   w[PH_SPLIT] = put(sp.data(), sp_words);
   put(table.data(), table.size());
@@ -408,7 +414,6 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
   w[PH_NSEQ] = n;
   w[PH_PAGES] = c.pages;
   w[PH_NDEC] = (int)di.size();
-  w[PH_NDSEQ] = (int)ds.size();
   w[PH_NPRE] = (int)pi.size();
   w[PH_NSPLIT] = (int)sp.size();
   w[PH_ROW0] = at_row0;

@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 ROOT = Path(__file__).resolve().parents[1]
-HDR = dict(ROWS=0, NSEQ=1, PAGES=4, NDEC=5, NDSEQ=6, NPRE=7, NSPLIT=8, ROW0=9, POS0=10, TOFF=11, DSEQ=12,
+HDR = dict(ROWS=0, NSEQ=1, PAGES=4, NDEC=5, NPRE=7, NSPLIT=8, ROW0=9, POS0=10, TOFF=11,
            PITEM=13, SPLIT=14, WORDS=32)
 P = 64
 
@@ -300,18 +300,14 @@ def test_plans_cover_what_each_row_sees_once(shim, seed):
                 seen_pages[row + k] += pages
             return slot
 
-        dec = w[HDR["WORDS"]:][: 8 * w[HDR["NDEC"]]].reshape(-1, 8)
-        for row, pos, table, sp, wp, v0, v1, slot in dec.tolist():
+        dec = w[HDR["WORDS"]:][: 12 * w[HDR["NDEC"]]].reshape(-1, 12)
+        for row, pos, table, sp, wp, v0, v1, slot, first, parts, *_ in dec.tolist():
             walk(row, pos, 1, table, sp, wp, v0, v1, slot)
-            if slot >= 0:
-                assert slot < b[0] and slot not in slots
-                slots[slot] = row
-        ds = w[w[HDR["DSEQ"]]:][: 4 * w[HDR["NDSEQ"]]].reshape(-1, 4)
-        for row, first, n, _ in ds.tolist():
-            assert (n > 1) == (first in slots and slots[first] == row) or n == 1
-            if n > 1:
-                assert all(slots.pop(first + k) == row for k in range(n))
-        assert not slots
+            assert first <= slot < first + parts and slot < b[0] and slot not in slots
+            slots[slot] = (row, first, parts)
+        for slot, (row, first, parts) in slots.items():
+            assert all(slots[first + k] == (row, first, parts) for k in range(parts))
+        slots.clear()
         pre = w[w[HDR["PITEM"]]:][: 12 * w[HDR["NPRE"]]].reshape(-1, 12)
         for row, pos, n, table, sp, wp, v0, v1, slot, *_ in pre.tolist():
             assert 1 <= n <= tile
