@@ -311,7 +311,7 @@ struct PkvAttnArgs {
   void* out;             // (rows, nh, hd)
   int window, sinks;     // window 0: every key up to the query's own
   float scale;
-  int ndec, npre, nsplit;   // the plan's counts when the call was made
+  int ndec, nwork, nsplit;   // the plan's counts when the call was made
   int captured;          // into a graph, whose replays may need joins that this plan does not
   uint32_t* tickets;     // (slots, nkv), 0 between launches
   float* dec_ml;         // (slots, nkv, rep, 2)

@@ -35,7 +35,7 @@ struct fmd_pkv {
   DevBuf pool;
   // the current plan
   bool planned = false;
-  int rows = 0, ndec = 0, npre = 0, nsplit = 0;
+  int rows = 0, ndec = 0, nwork = 0, nsplit = 0;
   DevBuf plan;
   PkvBounds most{};
   int32_t* stage[2] = {nullptr, nullptr};   // pinned; a slot is rewritten once its upload has passed
@@ -164,7 +164,7 @@ int pkv_attention(fmd_pkv* c, int layer, const void* q, void* ctx) {
   a.sinks = c->tab.sinks;
   a.scale = d->scale;
   a.ndec = c->ndec;
-  a.npre = c->npre;
+  a.nwork = c->nwork;
   a.nsplit = c->nsplit;
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   HIPCHK(hipStreamIsCapturing(d->stream, &cap));
@@ -384,7 +384,7 @@ extern "C" int fmd_pkv_plan(fmd_pkv* c, int n, const int32_t* seqs, const int32_
     c->slot ^= 1;
     c->rows = w[PH_ROWS];
     c->ndec = w[PH_NDEC];
-    c->npre = w[PH_NPRE];
+    c->nwork = w[PH_NWORK];
     c->nsplit = w[PH_NSPLIT];
     c->planned = true;
     return 0;

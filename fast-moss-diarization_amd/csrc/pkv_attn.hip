@@ -103,8 +103,16 @@ __device__ __forceinline__ void load_terms(const void* q, size_t at, bool ok, u3
   }
 }
 
-__device__ __forceinline__ const uint8_t* pool_of(const int32_t* plan) {
-  return (const uint8_t*)(((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL]);
+// Global memory by its address space: through a generic pointer the loads would
+// be flat ones, which LDS waits wait for, too.
+typedef const __attribute__((address_space(1))) uint8_t* gmem_t;
+typedef const __attribute__((address_space(1))) u32x4* gmem16_t;
+
+// The plan, which no kernel that reads it here writes: scalar loads.
+typedef const __attribute__((address_space(4))) int32_t* plan_t;
+__device__ __forceinline__ plan_t plan_of(const int32_t* p) { return (plan_t)(uint64_t)(uintptr_t)p; }
+__device__ __forceinline__ gmem_t pool_of(plan_t plan) {
+  return (gmem_t)(((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL]);
 }
 
 // Words that one work-group leaves for another of the same launch.
@@ -118,11 +126,6 @@ __device__ __forceinline__ float get(const float* p) {
 // ---- one new token --------------------------------------------------------
 
 constexpr int kDecWaves = 4;
-
-// The plan, which no kernel that reads it here writes: scalar loads, whose
-// counter the waits for the copies below do not share.
-typedef const __attribute__((address_space(4))) int32_t* plan_t;
-__device__ __forceinline__ plan_t plan_of(const int32_t* p) { return (plan_t)(uint64_t)(uintptr_t)p; }
 
 template <int A, int REP>
 __global__ void __launch_bounds__(64 * kDecWaves, 2) pkv_decode_kernel(PkvAttnArgs a) {
@@ -150,9 +153,8 @@ __global__ void __launch_bounds__(64 * kDecWaves, 2) pkv_decode_kernel(PkvAttnAr
   const float c2 = a.scale * kLog2e;
   const int n_items = plan[PH_NDEC];
   const size_t stride = (size_t)a.nkv * kPkvHeadBytes;       // bytes of a page
-  const uint8_t* layer =
-      (const uint8_t*)(((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL]) +
-      (size_t)a.layer * plan[PH_PAGES] * stride + (size_t)head * kPkvHeadBytes;
+  const uint8_t* layer = (const uint8_t*)(uint64_t)(pool_of(plan) + (size_t)a.layer * plan[PH_PAGES] * stride +
+                                                   (size_t)head * kPkvHeadBytes);
   uint8_t* const mine = &sPage[w][0];
   const uint32_t lds = lds_addr(mine);
   // Copy j < 4 brings the K codes of tokens 16 j .. 16 j + 15, j + 4 their V
@@ -247,11 +249,12 @@ __global__ void __launch_bounds__(64 * kDecWaves, 2) pkv_decode_kernel(PkvAttnAr
       const bool full = kb + kPkvPage - 1 <= item.pos &&
                         (a.window == 0 || kb > item.pos - a.window || kb + kPkvPage <= a.sinks);
       if (!full) {
+        const int behind = a.window ? item.pos - a.window : -1;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int j = kb + 16 * g + e;
-          if (j > item.pos || (a.window != 0 && j <= item.pos - a.window && j >= a.sinks))
-            s[e >> 2][e & 3] = -INFINITY;
+          const bool hidden = (j > item.pos) | ((j <= behind) & (j >= a.sinks));
+          s[e >> 2][e & 3] = hidden ? -INFINITY : s[e >> 2][e & 3];
         }
       }
       float bm = s[0][0];
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, 2) pkv_decode_kernel(PkvAttnAr
 // Waves of a work-group and sets of 16 positions of a wave.
 template <int A, int REP> struct PreShape {
   static constexpr int QS = A == ACT_F32 ? 1 : 2;
-  static constexpr int NW = REP == 1 ? 4 : 8;
+  static constexpr int NW = 4;
   static constexpr int TP = 16 * QS * (NW / REP);   // positions of a tile
 };
 
@@ -437,7 +440,7 @@ __device__ __forceinline__ int swk(int t) { return t & 15; }
 __device__ __forceinline__ int swv(int t) { return (t & 7) << 1; }
 
 template <int A, int REP>
-__global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kernel(PkvAttnArgs a) {
+__global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW), 2) pkv_prefill_kernel(PkvAttnArgs a) {
   constexpr bool F16 = A == ACT_F16;
   constexpr int NT = A == ACT_F32 ? 3 : 1;     // terms of q and of p
   constexpr int QS = PreShape<A, REP>::QS, NW = PreShape<A, REP>::NW, TP = PreShape<A, REP>::TP;
@@ -445,34 +448,46 @@ __global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kerne
   constexpr int BLK = kPkvPage * HD;
   __shared__ __attribute__((aligned(16))) uint16_t sK[2][BLK];
   __shared__ __attribute__((aligned(16))) uint16_t sV[2][BLK];
-  const int32_t* plan = a.plan;
+  const plan_t plan = plan_of(a.plan);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int qr = lane & 15, kg = lane >> 4;
   const int r = w % REP, half = w / REP, nh = a.nkv * REP;
   const float c2 = a.scale * kLog2e;
   const size_t stride = (size_t)a.nkv * kPkvHeadBytes;
-  const int n_units = plan[PH_NPRE] * a.nkv;
-  const uint8_t* pool = pool_of(plan) + (size_t)a.layer * plan[PH_PAGES] * stride;
+  const int n_work = plan[PH_NWORK], n_units = n_work * a.nkv;
+  const gmem_t pool = pool_of(plan) + (size_t)a.layer * plan[PH_PAGES] * stride;
 
   for (int un = blockIdx.x; un < n_units; un += gridDim.x) {
-    // Adjacent items of a KV head (a sequence's tiles) read the same pages:
-    // each XCD (work-groups are dealt round-robin) takes a contiguous run.
+    // Neighbours of a KV head (a sequence's tiles) read the same pages: each XCD
+    // (work-groups are dealt round-robin) takes a contiguous run.
     int unit = un;
     {
       const int per = n_units >> 3;
       if (un < 8 * per) unit = (un & 7) * per + (un >> 3);
     }
-    const int head = unit / plan[PH_NPRE];
-    const PkvPreItem item = ((const PkvPreItem*)(plan + plan[PH_PITEM]))[unit % plan[PH_NPRE]];
+    const int head = unit / n_work;
+    const plan_t work = plan + plan[PH_WORK] + unit % n_work;
+    for (int it = work[0], end = work[1]; it < end; ++it) {
+    const plan_t ip = plan + plan[PH_PITEM] + it * (int)(sizeof(PkvPreItem) / 4);
+    PkvPreItem item;
+    item.row = ip[0];
+    item.pos = ip[1];
+    item.n = ip[2];
+    item.table = ip[3];
+    item.sp = ip[4];
+    item.wp = ip[5];
+    item.v0 = ip[6];
+    item.v1 = ip[7];
+    item.slot = ip[8];
     const int rows = min(item.n, a.rows - item.row);
     if (rows <= 0) continue;
     const int h = head * REP + r;
-    const int32_t* table = plan + item.table;
-    const uint8_t* hbase = pool + (size_t)head * kPkvHeadBytes;
+    const plan_t table = plan + item.table;
+    const gmem_t hbase = pool + (size_t)head * kPkvHeadBytes;
     auto page_of = [&](int v) { return v < item.sp ? v : item.wp + (v - item.sp); };
     const int last = item.pos + item.n - 1;      // the tile's last position
 
-    int lim[QS];
+    int lim[QS], behind[QS];   // the last visible key, the last one behind the window
     u32x4 qf[QS][4][NT];
     float m2[QS], mr[QS];
     f32x4 o[QS][8], ls[QS];
@@ -481,6 +496,7 @@ __global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kerne
       const int my = 16 * (QS * half + qs) + qr;
       const bool ok = my < rows;
       lim[qs] = ok ? item.pos + my : item.pos;   // rows past the end see what the first does
+      behind[qs] = a.window ? lim[qs] - a.window : -1;
 #pragma unroll
       for (int ks = 0; ks < 4; ++ks)
         load_terms<A, NT>(a.q, ((size_t)(item.row + my) * nh + h) * HD + 32 * ks + 8 * kg, ok, qf[qs][ks]);
@@ -497,11 +513,11 @@ __global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kerne
     u32x4 raw[CH];
     int rsc[CH];
     auto fetch = [&](int v) {
-      const uint8_t* hp = hbase + (size_t)table[page_of(v)] * stride;
+      const gmem_t hp = hbase + (size_t)table[page_of(v)] * stride;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int x = i * NTH + tid, t = (x >> 2) & 63, b = x & 3;
-        raw[i] = *(const u32x4*)(hp + 16 * x);
+        raw[i] = *(gmem16_t)(hp + 16 * x);
         rsc[i] = hp[x < 256 ? kPkvKs + 64 * b + 4 * (4 * (t >> 4) + (t & 3)) + ((t >> 2) & 3)
                             : kPkvVs + 64 * b + t];
       }
@@ -519,45 +535,65 @@ __global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kerne
         int byte = rsc[i];
         if (isv && byte == 255) byte = 127;
         const float sc = __builtin_bit_cast(float, (uint32_t)byte << 23);
-        const bool dead = kb + t > last;
+        if (kb + t > last) raw[i] = u32x4{0, 0, 0, 0};
         uint16_t* row = (isv ? sV[buf] : sK[buf]) + t * HD;
         const int sw = isv ? swv(t) : swk(t);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          u32x4 e = widen8<F16>(raw[i][j], sc);
-          if (dead) e = u32x4{0, 0, 0, 0};
-          *(u32x4*)(row + (((4 * b + j) ^ sw) << 3)) = e;
-        }
+        for (int j = 0; j < 4; ++j) *(u32x4*)(row + (((4 * b + j) ^ sw) << 3)) = widen8<F16>(raw[i][j], sc);
       }
     };
-    if (item.v0 < item.v1) {
-      fetch(item.v0);
-      stage(item.v0, 0);
-    }
+    fetch(item.v0);   // an item has a page at least
+    stage(item.v0, 0);
     __syncthreads();
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     for (int v = item.v0, buf = 0; v < item.v1; ++v, buf ^= 1) {
-      const bool more = v + 1 < item.v1;
-      if (more) fetch(v + 1);
+      const int after = min(v + 1, item.v1 - 1);   // the last page once more, so that no branch is needed
+      fetch(after);
       const int kb = page_of(v) * kPkvPage;
       const uint16_t* kbuf = sK[buf];
       const uint16_t* vbuf = sV[buf];
+      // LDS reads go out a group ahead of the products that use them (a group is
+      // 8 products, 128 cycles; a read takes about as long): K by tile, V by
+      // half-block of tokens and half of the dims.  The scheduling barriers keep
+      // the compiler from pulling them back together.
       f32x4 s[4][QS];
+      u32x4 kf[2][4];
+      auto read_k = [&](int mt) {
+        const int t = 16 * mt + qr;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+          kf[mt & 1][ks] = *(const u32x4*)(kbuf + t * HD + (((4 * ks + kg) ^ swk(t)) << 3));
+      };
+      s16x4 vf[2][4][2];
+      auto read_v = [&](int gr) {
+        const int t = 32 * (gr >> 1) + 4 * kg + (qr >> 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 4 * (gr & 1) + i;
+          const uint16_t* at = vbuf + t * HD + (((2 * d + ((qr & 3) >> 1)) ^ swv(t)) << 3) + 4 * (qr & 1);
+          vf[gr & 1][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+          vf[gr & 1][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * HD));
+        }
+      };
+      read_k(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
+        if (mt < 3) read_k(mt + 1);
+        else read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int qs = 0; qs < QS; ++qs) s[mt][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-          const int t = 16 * mt + qr;
-          const u32x4 ka = *(const u32x4*)(kbuf + t * HD + (((4 * ks + kg) ^ swk(t)) << 3));
+        for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
           for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[mt][qs] = mfma<F16>(ka, qf[qs][ks][n], s[mt][qs]);
-        }
+            for (int n = 0; n < NT; ++n) s[mt][qs] = mfma<F16>(kf[mt & 1][ks], qf[qs][ks][n], s[mt][qs]);
+        __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       const bool full = kb + kPkvPage - 1 <= item.pos &&
                         (a.window == 0 || kb > last - a.window || kb + kPkvPage <= a.sinks);
       bool grow = false;
@@ -568,8 +604,8 @@ __global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kerne
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const int j = kb + 16 * (e >> 2) + 4 * kg + (e & 3);
-            if (j > lim[qs] || (a.window != 0 && j <= lim[qs] - a.window && j >= a.sinks))
-              s[e >> 2][qs][e & 3] = -INFINITY;
+            const bool hidden = (j > lim[qs]) | ((j <= behind[qs]) & (j >= a.sinks));
+            s[e >> 2][qs][e & 3] = hidden ? -INFINITY : s[e >> 2][qs][e & 3];
           }
         }
         bm[qs] = s[0][qs][0];
@@ -593,43 +629,53 @@ __global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kerne
       }
       // O^T += V^T P^T over tokens 32 hb .. 32 hb + 31: k-slot i of group kg is
       // token 32 hb + 4 kg + i (i < 4) or 32 hb + 16 + 4 kg + i - 4, where S^T has them
+      u32x4 pb[2][QS][NT];
+      auto weigh = [&](int hb, int qs) {
 #pragma unroll
-      for (int hb = 0; hb < 2; ++hb) {
-        u32x4 pb[QS][NT];
+        for (int e = 0; e < 8; e += 2) {
+          const f32x4 x = s[2 * hb + (e >> 2)][qs];
+          float p0 = __builtin_amdgcn_exp2f(fmaf(x[e & 3], c2, -mr[qs]));
+          float p1 = __builtin_amdgcn_exp2f(fmaf(x[(e & 3) + 1], c2, -mr[qs]));
 #pragma unroll
-        for (int qs = 0; qs < QS; ++qs)
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const f32x4 x = s[2 * hb + (e >> 2)][qs];
-            float p0 = __builtin_amdgcn_exp2f(fmaf(x[e & 3], c2, -mr[qs]));
-            float p1 = __builtin_amdgcn_exp2f(fmaf(x[(e & 3) + 1], c2, -mr[qs]));
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              pb[qs][n][e / 2] = pack2<F16>(p0, p1);
-              if (n + 1 < NT) {
-                p0 -= rd_bf16(p0);
-                p1 -= rd_bf16(p1);
-              }
+          for (int n = 0; n < NT; ++n) {
+            pb[hb][qs][n][e / 2] = pack2<F16>(p0, p1);
+            if (n + 1 < NT) {
+              p0 -= rd_bf16(p0);
+              p1 -= rd_bf16(p1);
             }
           }
+        }
+      };
 #pragma unroll
-        for (int qs = 0; qs < QS; ++qs)
+      for (int qs = 0; qs < QS; ++qs) weigh(0, qs);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) ls[qs] = mfma<F16>(ones, pb[qs][n], ls[qs]);
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const int t = 32 * hb + 4 * kg + (qr >> 2);
-          const uint16_t* at = vbuf + t * HD + (((2 * d + ((qr & 3) >> 1)) ^ swv(t)) << 3) + 4 * (qr & 1);
-          const s16x4 r1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-          const s16x4 r2 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * HD));
-          const u32x4 va = __builtin_bit_cast(u32x4, __builtin_shufflevector(r1, r2, 0, 1, 2, 3, 4, 5, 6, 7));
+      for (int gr = 0; gr < 4; ++gr) {
+        const int hb = gr >> 1;
+        if (gr < 3) read_v(gr + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if ((gr & 1) == 0) {
 #pragma unroll
           for (int qs = 0; qs < QS; ++qs)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) o[qs][d] = mfma<F16>(va, pb[qs][n], o[qs][d]);
+            for (int n = 0; n < NT; ++n) ls[qs] = mfma<F16>(ones, pb[hb][qs][n], ls[qs]);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 4 * (gr & 1) + i;
+          const u32x4 va = __builtin_bit_cast(
+              u32x4, __builtin_shufflevector(vf[gr & 1][i][0], vf[gr & 1][i][1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[qs][d] = mfma<F16>(va, pb[hb][qs][n], o[qs][d]);
+        }
+        // the second half's exponentials between the first half's products
+        if (gr < 2 && gr < QS) weigh(1, gr);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (more) stage(v + 1, buf ^ 1);
+      __builtin_amdgcn_s_setprio(0);
+      stage(after, buf ^ 1);
       __syncthreads();
     }
 #pragma unroll
@@ -661,6 +707,7 @@ __global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW)) pkv_prefill_kerne
       }
     }
     __syncthreads();
+    }
   }
 }
 
@@ -706,8 +753,8 @@ template <int A, int REP>
 hipError_t launch_rep(const PkvAttnArgs& a, hipStream_t s) {
   if (a.ndec > 0)
     hipLaunchKernelGGL((pkv_decode_kernel<A, REP>), dim3(a.ndec, a.nkv), dim3(64 * kDecWaves), 0, s, a);
-  if (a.npre > 0) {
-    hipLaunchKernelGGL((pkv_prefill_kernel<A, REP>), dim3(a.npre * a.nkv),
+  if (a.nwork > 0) {
+    hipLaunchKernelGGL((pkv_prefill_kernel<A, REP>), dim3(a.nwork * a.nkv),
                        dim3(64 * PreShape<A, REP>::NW), 0, s, a);
     if (a.nsplit > 0 || a.captured)
       hipLaunchKernelGGL((pkv_prefill_join_kernel<A, REP>),

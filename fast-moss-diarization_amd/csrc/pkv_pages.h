@@ -34,12 +34,13 @@ enum PkvHdr {
   PH_POOL = 2,     // pool address, low and high word
   PH_PAGES = 4,    // pages of the pool (the layer stride)
   PH_NDEC = 5,     // decode items, in front of the other sections
-  PH_NPRE = 7,     // many-token items
+  PH_NWORK = 7,    // work-groups per KV head of the many-token rows
   PH_NSPLIT = 8,   // many-token tiles cut into several items
   PH_ROW0 = 9,     // offset: first row of each sequence, and the row count
   PH_POS0 = 10,    // offset: position of that row
   PH_TOFF = 11,    // offset: where the sequence's page ids are
   PH_PITEM = 13,   // offset: PkvPreItem entries
+  PH_WORK = 6,     // offset: first item of each of them, and the item count
   PH_SPLIT = 14,   // offset: PkvSplit entries
   PH_WORDS = 32
 };
@@ -295,16 +296,15 @@ class PkvPages {
 
 // ---- the plan ----
 
-// Work-groups that the attention's items are cut for, over all KV heads, and
-// the pages of an item at least (a decode work-group's four waves take one each).
+// Work-groups that the attention is cut for, over all KV heads (two on each CU),
+// and the pages of a decode item and a many-token work-group at least.
 constexpr int kPkvDecGroups = 512, kPkvPreGroups = 512;
-constexpr int kPkvDecMinPages = 4, kPkvPreMinPages = 8;
+constexpr int kPkvDecMinPages = 8, kPkvPreMinPages = 8;
 
 // What a plan takes at most.  Decode: an item's pages are at least all rows'
 // pages over kPkvDecGroups / nkv, so there are at most that many items and one
-// more per row.  Many tokens: a tile is cut only when it has more pages than
-// that, so fewer than kPkvPreGroups / nkv tiles are, into at most twice as many
-// items.
+// more per row.  Many tokens: the tiles' pages, one tile after another, are cut
+// into equal runs for the work-groups; a cut adds an item and makes two partial.
 struct PkvBounds {
   int dec_items, tiles, pre_slots;
   size_t words;
@@ -316,7 +316,7 @@ inline PkvBounds pkv_bounds(int nkv, int max_seqs, int max_rows, int max_len, in
   b.pre_slots = 2 * (kPkvPreGroups / nkv + 1);
   b.words = PH_WORDS + ((size_t)b.dec_items * sizeof(PkvDecItem) +
                         (size_t)(b.tiles + b.pre_slots) * sizeof(PkvPreItem) +
-                        (size_t)b.pre_slots * sizeof(PkvSplit)) / 4 +
+                        (size_t)b.pre_slots * (sizeof(PkvSplit) + 4)) / 4 +
             3 * (size_t)max_seqs + 1 + (size_t)max_seqs * pkv_ceil(max_len, kPkvPage);
   return b;
 }
@@ -356,8 +356,9 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
   for (const Row& r : order) dec_rows += r.n == 1;
   while ((int64_t)dec_rows * nkv <= kPkvDecGroups && dec_items() * nkv > kPkvDecGroups)
     dec_per += std::max(1, dec_per / 16);
-  const int pre_per = std::max(kPkvPreMinPages, pkv_ceil(pre_pages * nkv, kPkvPreGroups));
-  int dec_slots = 0, pre_slots = 0;
+  const int pre_per = std::max(kPkvPreMinPages, pkv_ceil(pre_pages, std::max(1, kPkvPreGroups / nkv)));
+  int dec_slots = 0, pre_slots = 0, room = pre_per;   // pages that the work-group at hand still takes
+  std::vector<int32_t> work(1, 0);
   for (int i = 0; i < n; ++i) {
     const Row& r = order[i];
     toff[i] = (int)table.size();
@@ -373,15 +374,26 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
       for (int p = 0; p < r.n; p += tile) {
         const int m = std::min(tile, r.n - p);
         const PkvPages::Visible v = c.visible(r.pos + p, r.pos + p + m - 1);
-        const int per = pkv_ceil(v.n, pkv_ceil(v.n, pre_per)), parts = pkv_ceil(v.n, per);
-        if (parts > 1) sp.push_back({r.row + p, m, pre_slots, parts});
-        for (int k = 0; k < parts; ++k)
-          pi.push_back({r.row + p, r.pos + p, m, i, v.sp, v.wp, k * per, std::min((k + 1) * per, v.n),
-                        parts > 1 ? pre_slots + k : -1, {0, 0, 0}});
-        pre_slots += parts > 1 ? parts : 0;
+        const bool whole = v.n <= room;
+        int parts = 0;
+        for (int v0 = 0; v0 < v.n; ++parts) {
+          const int k = std::min(room, v.n - v0);
+          pi.push_back({r.row + p, r.pos + p, m, i, v.sp, v.wp, v0, v0 + k, whole ? -1 : pre_slots + parts, {0, 0, 0}});
+          v0 += k;
+          room -= k;
+          if (room == 0) {
+            work.push_back((int)pi.size());
+            room = pre_per;
+          }
+        }
+        if (!whole) {
+          sp.push_back({r.row + p, m, pre_slots, parts});
+          pre_slots += parts;
+        }
       }
     }
   }
+  if (work.back() != (int)pi.size()) work.push_back((int)pi.size());
   std::vector<int32_t> w(PH_WORDS, 0);
   auto section = [&](size_t words) {
     const int at = (int)w.size();
@@ -396,7 +408,7 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
   // the sections' sizes are known: the tables come last, behind `table_at`
   const size_t di_words = di.size() * sizeof(PkvDecItem) / 4,
                pi_words = pi.size() * sizeof(PkvPreItem) / 4, sp_words = sp.size() * sizeof(PkvSplit) / 4;
-  const int table_at = (int)(PH_WORDS + di_words + 3 * (size_t)n + 1 + pi_words + sp_words);
+  const int table_at = (int)(PH_WORDS + di_words + 3 * (size_t)n + 1 + pi_words + work.size() + sp_words);
   for (PkvDecItem& x : di) x.table = table_at + toff[x.table];
   for (PkvPreItem& x : pi) x.table = table_at + toff[x.table];
   put(di.data(), di_words);
@@ -408,13 +420,14 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
   }
   w[at_row0 + n] = rows;
   w[PH_PITEM] = put(pi.data(), pi_words);
+  w[PH_WORK] = put(work.data(), work.size());
   w[PH_SPLIT] = put(sp.data(), sp_words);
   put(table.data(), table.size());
   w[PH_ROWS] = rows;
   w[PH_NSEQ] = n;
   w[PH_PAGES] = c.pages;
   w[PH_NDEC] = (int)di.size();
-  w[PH_NPRE] = (int)pi.size();
+  w[PH_NWORK] = (int)work.size() - 1;
   w[PH_NSPLIT] = (int)sp.size();
   w[PH_ROW0] = at_row0;
   w[PH_POS0] = at_pos0;

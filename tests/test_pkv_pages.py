@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 ROOT = Path(__file__).resolve().parents[1]
-HDR = dict(ROWS=0, NSEQ=1, PAGES=4, NDEC=5, NPRE=7, NSPLIT=8, ROW0=9, POS0=10, TOFF=11,
+HDR = dict(ROWS=0, NSEQ=1, PAGES=4, NDEC=5, WORK=6, NWORK=7, NSPLIT=8, ROW0=9, POS0=10, TOFF=11,
            PITEM=13, SPLIT=14, WORDS=32)
 P = 64
 
@@ -308,7 +308,11 @@ def test_plans_cover_what_each_row_sees_once(shim, seed):
         for slot, (row, first, parts) in slots.items():
             assert all(slots[first + k] == (row, first, parts) for k in range(parts))
         slots.clear()
-        pre = w[w[HDR["PITEM"]]:][: 12 * w[HDR["NPRE"]]].reshape(-1, 12)
+        work = w[w[HDR["WORK"]]:][: w[HDR["NWORK"]] + 1].tolist()
+        assert work[0] == 0 and work == sorted(set(work)) and len(work) <= b[2] + 1
+        pre = w[w[HDR["PITEM"]]:][: 12 * work[-1]].reshape(-1, 12)
+        loads = [int((pre[x:y, 7] - pre[x:y, 6]).sum()) for x, y in zip(work, work[1:])]
+        assert len(set(loads[:-1])) <= 1 and (not loads or loads[-1] <= loads[0])
         for row, pos, n, table, sp, wp, v0, v1, slot, *_ in pre.tolist():
             assert 1 <= n <= tile
             walk(row, pos, n, table, sp, wp, v0, v1, slot)
