@@ -229,6 +229,8 @@ extern "C" int fmd_dec_destroy(fmd_dec* d) {
     if (p) hipFree(p);
   d->staging.release();
   d->staging2.release();
+  d->pkv_cos.release();
+  d->pkv_sin.release();
   d->ws.release_all();
   if (d->host_mirror) hipHostFree(d->host_mirror);
   if (d->host_stage) hipHostFree(d->host_stage);

@@ -77,6 +77,7 @@ struct fmd_dec {
   void* sin = nullptr;
   bool embed_set = false, norm_set = false, lm_head_set = false, lm_head_explicit = false;
   DevBuf staging, staging2;
+  DevBuf pkv_cos, pkv_sin;   // rotation tables of the paged caches' appends (the first cache makes them)
   Workspace ws;
   int32_t* host_mirror = nullptr;  // host-mapped copy of the greedy state and the attention error code
   void* host_stage = nullptr;      // pinned host staging of prefill chunk tables

@@ -275,8 +275,17 @@ int gemv_logits_nparts(int act, bool q8, bool norm, int hidden, int out_rows);
 
 // ---- paged 4-bit KV cache (pkv_rows.hip, pkv_attn.hip; layouts in pkv_pages.h) ----
 
+// Rotation tables (positions, 64) of the append: cosine and sine of the f32
+// angles pos * inv[i], rounded once to f32 and then to the activation dtype.
+struct RopeFreqs {
+  float inv[64];
+};
+hipError_t launch_pkv_rope(int act, const RopeFreqs& f, int positions, void* cos, void* sin,
+                           hipStream_t s);
+
 struct PkvRowArgs {
   const int32_t* plan;
+  const int32_t* far;    // the rows of plans of more than kPkvDirect
   int layer, nh, nkv;
   int rows;              // rows of the caller's buffers: rows past it are left alone
   const void* x;         // append: (rows, (nh + 2 nkv) hd); write: K (rows, nkv, hd)

@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <exception>
 #include <string>
@@ -108,6 +109,21 @@ int sync_own(fmd_dec* d) {
   return 0;
 }
 
+int make_tables(fmd_dec* d) {
+  if (d->pkv_cos.p && d->pkv_sin.p) return 0;
+  const size_t bytes = (size_t)d->max_len * (d->hd / 2) * d->esz;
+  CHK(d->pkv_cos.ensure(bytes));
+  RopeFreqs f;
+  for (int i = 0; i < 64; ++i)   // as fmd_dec_create
+    f.inv[i] = (float)(1.0 / std::pow(d->cfg.rope_theta, 2.0 * (double)i / (double)d->hd));
+  int rc = d->pkv_sin.ensure(bytes);
+  if (!rc && launch_pkv_rope(d->act, f, d->max_len, d->pkv_cos.p, d->pkv_sin.p, d->stream) != hipSuccess) {
+    d->pkv_sin.release();
+    rc = fmd_fail(FMD_ERR_HIP, "rotation tables failed");
+  }
+  return rc;
+}
+
 int check_op(fmd_dec* d, const fmd_pkv* c, int layer) {
   if (!d || !c) return fmd_fail(FMD_ERR_ARG, "null handle");
   if (c->dec != d) return fmd_fail(FMD_ERR_STATE, "cache belongs to another decoder");
@@ -124,6 +140,7 @@ PkvRowArgs row_args(const fmd_pkv* c, int layer) {
   const fmd_dec* d = c->dec;
   PkvRowArgs a{};
   a.plan = c->plan.as<int32_t>();
+  a.far = a.plan + c->most.rows_at;
   a.layer = layer;
   a.nh = d->nh;
   a.nkv = d->nkv;
@@ -142,8 +159,8 @@ int pkv_append(fmd_pkv* c, int layer, const void* qkv, void* q) {
   a.x = qkv;
   a.qn_w = d->layers[layer].q_norm;
   a.kn_w = d->layers[layer].k_norm;
-  a.cos = d->cos;
-  a.sin = d->sin;
+  a.cos = d->pkv_cos.p;
+  a.sin = d->pkv_sin.p;
   a.q_out = q;
   HIPCHK(launch_pkv_append(d->act, a, d->stream));
   return 0;
@@ -223,7 +240,8 @@ extern "C" int fmd_pkv_create(fmd_dec* d, int pages, int max_seqs, int max_rows,
   c->most = pkv_bounds(d->nkv, max_seqs, max_rows, d->max_len, tile);
   const size_t dec_units = (size_t)c->most.dec_items * d->nkv * d->rep;
   const size_t pre_units = max_rows > 1 ? (size_t)c->most.pre_slots * d->nkv * tile * d->rep : 0;
-  rc = c->pool.ensure(fmd_pkv_bytes(d, pages));
+  rc = make_tables(d);
+  if (!rc) rc = c->pool.ensure(fmd_pkv_bytes(d, pages));
   if (!rc) rc = c->plan.ensure(c->most.words * 4);
   if (!rc) rc = c->tickets.ensure((size_t)c->most.dec_items * d->nkv * 4);
   if (!rc) rc = c->dec_ml.ensure(dec_units * 8);
@@ -370,9 +388,10 @@ extern "C" int fmd_pkv_plan(fmd_pkv* c, int n, const int32_t* seqs, const int32_
     CHK(told(c, c->tab.extend(n, seqs, counts, &l)));
     CHK(drop_plan(c));
     CHK(copy_pairs(c, l, c->pool.p, c->tab.pages, c->pool.p, c->tab.pages));
+    std::vector<int32_t> far;
     std::vector<int32_t> w =
-        pkv_build_plan(c->tab, d->nkv, pkv_tile_positions(d->act, d->rep), n, seqs, counts);
-    if (w.size() > c->most.words || w[PH_NDEC] > c->most.dec_items)
+        pkv_build_plan(c->tab, d->nkv, pkv_tile_positions(d->act, d->rep), n, seqs, counts, &far);
+    if (w.size() > c->most.rows_at || w[PH_NDEC] > c->most.dec_items)
       return fmd_fail(FMD_ERR_STATE, "plan larger than its buffer");
     const uint64_t pool = (uint64_t)(uintptr_t)c->pool.p;
     w[PH_POOL] = (int32_t)(uint32_t)pool;
@@ -380,6 +399,12 @@ extern "C" int fmd_pkv_plan(fmd_pkv* c, int n, const int32_t* seqs, const int32_
     HIPCHK(hipEventSynchronize(c->staged[c->slot]));
     std::memcpy(c->stage[c->slot], w.data(), w.size() * 4);
     HIPCHK(hipMemcpyAsync(c->plan.p, c->stage[c->slot], w.size() * 4, hipMemcpyHostToDevice, d->stream));
+    if (!far.empty()) {
+      const size_t at = c->most.rows_at;
+      std::memcpy(c->stage[c->slot] + at, far.data(), far.size() * 4);
+      HIPCHK(hipMemcpyAsync(c->plan.as<int32_t>() + at, c->stage[c->slot] + at, far.size() * 4,
+                            hipMemcpyHostToDevice, d->stream));
+    }
     HIPCHK(hipEventRecord(c->staged[c->slot], d->stream));
     c->slot ^= 1;
     c->rows = w[PH_ROWS];

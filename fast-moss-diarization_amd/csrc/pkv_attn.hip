@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, 2) pkv_decode_kernel(PkvAttnAr
   };
 
   for (int it = blockIdx.x; it < n_items; it += gridDim.x) {
-    const plan_t ip = plan + PH_WORDS + it * (int)(sizeof(PkvDecItem) / 4);
+    const plan_t ip = plan + PH_ITEMS + it * (int)(sizeof(PkvDecItem) / 4);
     PkvDecItem item;
     item.row = ip[0];
     item.pos = ip[1];
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(64 * kDecWaves, 2) pkv_decode_kernel(PkvAttnAr
     auto page_of = [&](int v) { return v < item.sp ? v : item.wp + (v - item.sp); };
     auto id_of = [&](int v) { return table[page_of(min(v, item.v1 - 1))]; };   // read a step ahead
     const int first = item.v0 + w;
-    int id = id_of(first);
+    int id = ip[10 + w];
     {
       const uint8_t* q = (const uint8_t*)a.q + ((size_t)item.row * nh + head * REP) * (HD * ESZ);
 #pragma unroll

@@ -26,29 +26,30 @@ constexpr int kPkvPage = 64;
 constexpr int kPkvHeadBytes = 8704;
 constexpr int kPkvV = 4096, kPkvKs = 8192, kPkvVs = 8448;
 
-// The plan in device memory (32-bit words): the header, then the decode items,
-// and at header offsets the other sections.
+// The plan in device memory (32-bit words): the header, then position and page
+// of each row of a plan of at most kPkvDirect rows, then the decode items, and
+// at header offsets the other sections.  The rows of a larger plan are at
+// PkvBounds::rows_at: a second upload, which small plans do without.
+constexpr int kPkvDirect = 256;
 enum PkvHdr {
   PH_ROWS = 0,     // rows of the plan; 0 when there is no plan
-  PH_NSEQ = 1,
-  PH_POOL = 2,     // pool address, low and high word
-  PH_PAGES = 4,    // pages of the pool (the layer stride)
-  PH_NDEC = 5,     // decode items, in front of the other sections
-  PH_NWORK = 7,    // work-groups per KV head of the many-token rows
-  PH_NSPLIT = 8,   // many-token tiles cut into several items
-  PH_ROW0 = 9,     // offset: first row of each sequence, and the row count
-  PH_POS0 = 10,    // offset: position of that row
-  PH_TOFF = 11,    // offset: where the sequence's page ids are
-  PH_PITEM = 13,   // offset: PkvPreItem entries
-  PH_WORK = 6,     // offset: first item of each of them, and the item count
-  PH_SPLIT = 14,   // offset: PkvSplit entries
-  PH_WORDS = 32
+  PH_POOL = 1,     // pool address, low and high word
+  PH_PAGES = 3,    // pages of the pool (the layer stride)
+  PH_NDEC = 4,     // decode items, behind the rows
+  PH_NWORK = 5,    // work-groups per KV head of the many-token rows
+  PH_NSPLIT = 6,   // many-token tiles in several items
+  PH_WORK = 7,     // offset: first item of each of those work-groups, and the item count
+  PH_PITEM = 8,    // offset: PkvPreItem entries
+  PH_SPLIT = 9,    // offset: PkvSplit entries
+  PH_WORDS = 32,
+  PH_ITEMS = PH_WORDS + 2 * kPkvDirect
 };
 // The visible pages of an item's queries, in order: pages [0, sp) (the sinks),
 // then pages wp, wp + 1, ..; v counts through both.
 struct PkvDecItem {
   int32_t row, pos, table, sp, wp, v0, v1;
   int32_t slot, first, parts;                      // its partial slot, of first .. first + parts - 1 of its row
+  int32_t id[4];                                   // the first pages of its four waves
   int32_t pad[2];
 };
 struct PkvPreItem {
@@ -307,6 +308,7 @@ constexpr int kPkvDecMinPages = 8, kPkvPreMinPages = 8;
 // into equal runs for the work-groups; a cut adds an item and makes two partial.
 struct PkvBounds {
   int dec_items, tiles, pre_slots;
+  size_t rows_at;   // the rows of plans of more than kPkvDirect
   size_t words;
 };
 inline PkvBounds pkv_bounds(int nkv, int max_seqs, int max_rows, int max_len, int tile) {
@@ -314,17 +316,19 @@ inline PkvBounds pkv_bounds(int nkv, int max_seqs, int max_rows, int max_len, in
   b.dec_items = kPkvDecGroups / nkv + max_seqs + 1;
   b.tiles = max_rows / tile + max_seqs;
   b.pre_slots = 2 * (kPkvPreGroups / nkv + 1);
-  b.words = PH_WORDS + ((size_t)b.dec_items * sizeof(PkvDecItem) +
-                        (size_t)(b.tiles + b.pre_slots) * sizeof(PkvPreItem) +
-                        (size_t)b.pre_slots * (sizeof(PkvSplit) + 4)) / 4 +
-            3 * (size_t)max_seqs + 1 + (size_t)max_seqs * pkv_ceil(max_len, kPkvPage);
+  b.rows_at = PH_ITEMS + ((size_t)b.dec_items * sizeof(PkvDecItem) +
+                          (size_t)(b.tiles + b.pre_slots) * sizeof(PkvPreItem) +
+                          (size_t)b.pre_slots * (sizeof(PkvSplit) + 4)) / 4 +
+              (size_t)max_seqs * pkv_ceil(max_len, kPkvPage);
+  b.words = b.rows_at + (max_rows > kPkvDirect ? 2 * (size_t)max_rows : 0);
   return b;
 }
 
 // The plan of the last counts[i] tokens of seqs[i], `tile` positions to a
-// many-token tile; the pool's address goes into the header later.
-inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile, int n,
-                                           const int32_t* seqs, const int32_t* counts) {
+// many-token tile; the pool's address goes into the header later.  The rows of a
+// plan of more than kPkvDirect are left in *far.
+inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile, int n, const int32_t* seqs,
+                                           const int32_t* counts, std::vector<int32_t>* far) {
   struct Row {
     int seq, row, pos, n;
   };
@@ -366,9 +370,15 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
     if (r.n == 1) {
       const PkvPages::Visible v = c.visible(r.pos, r.pos);
       const int per = pkv_ceil(v.n, pkv_ceil(v.n, dec_per)), parts = pkv_ceil(v.n, per);
-      for (int k = 0; k < parts; ++k)
-        di.push_back({r.row, r.pos, i, v.sp, v.wp, k * per, std::min((k + 1) * per, v.n), dec_slots + k,
-                      dec_slots, parts, {0, 0}});
+      for (int k = 0; k < parts; ++k) {
+        PkvDecItem x{r.row, r.pos, i, v.sp, v.wp, k * per, std::min((k + 1) * per, v.n), dec_slots + k,
+                     dec_slots, parts, {0, 0, 0, 0}, {0, 0}};
+        for (int j = 0; j < 4; ++j) {
+          const int at = std::min(x.v0 + j, x.v1 - 1);
+          x.id[j] = c.seqs[r.seq].pages[at < v.sp ? at : v.wp + at - v.sp];
+        }
+        di.push_back(x);
+      }
       dec_slots += parts;
     } else {
       for (int p = 0; p < r.n; p += tile) {
@@ -394,7 +404,7 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
     }
   }
   if (work.back() != (int)pi.size()) work.push_back((int)pi.size());
-  std::vector<int32_t> w(PH_WORDS, 0);
+  std::vector<int32_t> w(PH_ITEMS, 0);
   auto section = [&](size_t words) {
     const int at = (int)w.size();
     w.resize(w.size() + words);
@@ -408,29 +418,25 @@ inline std::vector<int32_t> pkv_build_plan(const PkvPages& c, int nkv, int tile,
   // the sections' sizes are known: the tables come last, behind `table_at`
   const size_t di_words = di.size() * sizeof(PkvDecItem) / 4,
                pi_words = pi.size() * sizeof(PkvPreItem) / 4, sp_words = sp.size() * sizeof(PkvSplit) / 4;
-  const int table_at = (int)(PH_WORDS + di_words + 3 * (size_t)n + 1 + pi_words + work.size() + sp_words);
+  const int table_at = (int)(PH_ITEMS + di_words + pi_words + work.size() + sp_words);
   for (PkvDecItem& x : di) x.table = table_at + toff[x.table];
   for (PkvPreItem& x : pi) x.table = table_at + toff[x.table];
   put(di.data(), di_words);
-  const int at_row0 = section(n + 1), at_pos0 = section(n), at_toff = section(n);
-  for (int i = 0; i < n; ++i) {
-    w[at_row0 + i] = order[i].row;
-    w[at_pos0 + i] = order[i].pos;
-    w[at_toff + i] = table_at + toff[i];
-  }
-  w[at_row0 + n] = rows;
   w[PH_PITEM] = put(pi.data(), pi_words);
   w[PH_WORK] = put(work.data(), work.size());
   w[PH_SPLIT] = put(sp.data(), sp_words);
   put(table.data(), table.size());
   w[PH_ROWS] = rows;
-  w[PH_NSEQ] = n;
   w[PH_PAGES] = c.pages;
   w[PH_NDEC] = (int)di.size();
   w[PH_NWORK] = (int)work.size() - 1;
   w[PH_NSPLIT] = (int)sp.size();
-  w[PH_ROW0] = at_row0;
-  w[PH_POS0] = at_pos0;
-  w[PH_TOFF] = at_toff;
+  far->assign(rows > kPkvDirect ? 2 * (size_t)rows : 0, 0);
+  int32_t* at = rows > kPkvDirect ? far->data() : w.data() + PH_WORDS;
+  for (const Row& r : order)
+    for (int k = 0; k < r.n; ++k) {
+      *at++ = r.pos + k;
+      *at++ = c.seqs[r.seq].pages[(r.pos + k) / kPkvPage];
+    }
   return w;
 }

@@ -12,9 +12,8 @@
 // a quarter); relative rms error of N(0, 1) blocks at 6 | 6.5 | 7 | 7.5 | 8:
 // .1155 | .1131 | .1119 | .1120 | .1151.
 //
-// K is computed in 64 bits (as fast as unpacked 32 bits on this device) and
-// rounded to 32: which code a value next to a border gets then does not depend
-// on the order of the mean's sum.  The wave's q heads take 32 bits.
+// K is computed to 64 bits and rounded to 32: which code a value next to a border
+// gets then does not depend on the order of the mean's sum.  q takes 32 bits.
 //
 // A token whose K or V of a head holds an infinity or a NaN gets scale 255 in
 // all eight blocks of that head: it reads back as NaN, and so does every
@@ -33,28 +32,22 @@ constexpr int HD = 128;
 template <int A> constexpr int kLo = A == ACT_F16 ? -23 : -64;
 template <int A> constexpr int kHi = A == ACT_F16 ? 13 : 64;
 
-// The sequence that holds `row`: the last one whose first row is <= row (one
-// with rows: a sequence without any starts where the next one does).
-__device__ __forceinline__ int seq_of(const int32_t* row0, int n, int row) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (row0[mid] <= row) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
+typedef const __attribute__((address_space(4))) int32_t* plan_t;   // scalar loads
+typedef __attribute__((address_space(1))) uint8_t* gmem_t;         // no flat ones
+typedef __attribute__((address_space(1))) uint32_t* gmem4_t;
 
-__device__ __forceinline__ uint8_t* pool_of(const int32_t* plan) {
-  return (uint8_t*)(((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL]);
-}
-
-// Head `h` of the page holding position `pos` of planned sequence `s`.
-__device__ __forceinline__ uint8_t* head_of(const int32_t* plan, int s, int pos, int layer, int nkv,
-                                            int h) {
-  const int page = plan[plan[plan[PH_TOFF] + s] + pos / kPkvPage];
-  return pool_of(plan) +
-         (((size_t)layer * plan[PH_PAGES] + page) * nkv + h) * (size_t)kPkvHeadBytes;
+// Where a row's token lies: its position, and the page.
+struct Place {
+  int pos;
+  gmem_t page;
+};
+__device__ __forceinline__ Place place_of(const PkvRowArgs& a, plan_t plan, int rows, int row) {
+  const plan_t at = (rows <= kPkvDirect ? plan + PH_WORDS : (plan_t)(uint64_t)a.far) + 2 * row;
+  const uint64_t pool = ((uint64_t)(uint32_t)plan[PH_POOL + 1] << 32) | (uint32_t)plan[PH_POOL];
+  Place p;
+  p.pos = at[0];
+  p.page = (gmem_t)pool + ((size_t)a.layer * plan[PH_PAGES] + at[1]) * a.nkv * (size_t)kPkvHeadBytes;
+  return p;
 }
 
 __device__ __forceinline__ int kscale_at(int t, int blk) {
@@ -119,43 +112,80 @@ __device__ __forceinline__ uint32_t codes8(const float* x, int byte) {
 
 // K (k) and V (v) of one token and head, 8 dims per lane of a 16-lane row.
 template <int A>
-__device__ __forceinline__ void store_kv(uint8_t* head, int t, int dc, const float* k, const float* v) {
+__device__ __forceinline__ void store_kv(gmem_t head, int t, int dc, const float* k, const float* v) {
   const uint32_t mk = quad_max_bits(k), mv = quad_max_bits(v);
   // any block of the row not finite: __ballot, then this row's 16 bits
   const uint64_t bad = __ballot(mk >= 0x7f800000u || mv >= 0x7f800000u);
   const bool nan = (bad >> (threadIdx.x & 48)) & 0xffffu;
   const int bk = scale_byte<A>(mk), bv = scale_byte<A>(mv);
-  *(uint32_t*)(head + t * 64 + dc * 4) = nan ? 0u : codes8(k, bk);
-  *(uint32_t*)(head + kPkvV + t * 64 + dc * 4) = nan ? 0u : codes8(v, bv);
+  *(gmem4_t)(head + t * 64 + dc * 4) = nan ? 0u : codes8(k, bk);
+  *(gmem4_t)(head + kPkvV + t * 64 + dc * 4) = nan ? 0u : codes8(v, bv);
   if ((dc & 3) == 0) {
     head[kPkvKs + kscale_at(t, dc >> 2)] = (uint8_t)(nan ? 255 : bk);
     head[kPkvVs + 64 * (dc >> 2) + t] = (uint8_t)(nan ? 255 : bv);
   }
 }
 
-__device__ __forceinline__ double row16_sum(double v) {
-  // lanes ^1, ^2, ^7 and ^15 of the 16-lane row, as the 32-bit sum takes them
-#pragma unroll
-  for (int m : {1, 2, 7, 15}) v += __shfl_xor(v, m);
-  return v;
+// The value of lane ^ 8 of the 16-lane row: dims 64 on.
+__device__ __forceinline__ float across(float v) { return FMD_DPP(v, 0x128); }
+
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
-// Norm and rotation of the 8 dims 8 dc .. of a head, in F.
-template <class F>
-__device__ __forceinline__ void norm_rope(const float* x, const float* g, const float* c,
-                                          const float* s, int dc, float eps, float* z) {
-  F ss = 0;
+// Norm and rotation of a q head's 8 dims 8 dc .., in 32 bits.
+__device__ __forceinline__ void norm_rope_q(const float* x, const float* g, const float* c,
+                                            const float* s, int dc, float eps, float* z) {
+  float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ss += (F)x[i] * (F)x[i];
+  for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
   ss = row16_sum(ss);
-  const F r = (F)1 / sqrt(ss / (F)HD + (F)eps);
-  F y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = (F)x[i] * r * (F)g[i];
+  const float r = __builtin_amdgcn_rsqf(ss * (1.f / HD) + eps);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const F o = __shfl_xor(y[i], 8);   // dim +- 64
-    z[i] = (float)(dc < 8 ? y[i] * (F)c[i] - o * (F)s[i] : y[i] * (F)c[i] + o * (F)s[i]);
+    const float y = x[i] * r * g[i], o = across(y);
+    z[i] = fmaf(y, c[i], dc < 8 ? -o * s[i] : o * s[i]);
+  }
+}
+
+// The same of a K head as if in 64 bits.  What is exact in 32 bits is done
+// there: a product of two 16-bit values, and of three bf16 ones (24 bits).
+template <int A>
+__device__ __forceinline__ void norm_rope_k(const float* x, const float* g, const float* c,
+                                            const float* s, int dc, float eps, float* z) {
+  double ss = 0.;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ss = fma((double)x[i], (double)x[i], ss);
+  ss += dpp64<0xB1>(ss);
+  ss += dpp64<0x4E>(ss);
+  ss += dpp64<0x141>(ss);
+  ss += dpp64<0x140>(ss);
+  // 1 / sqrt(m): the instruction's value, good to 2^-22 at least, and two Newton
+  // steps, each of which squares its error
+  const double m = fma(ss, 1. / HD, (double)eps);
+  double r = __builtin_amdgcn_rsq(m);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) r = fma(r, fma(-0.5 * m * r, r, 0.5), r);
+  const bool lo = dc < 8;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float xo = across(x[i]), go = across(g[i]);
+    double a, b;
+    if constexpr (A == ACT_BF16) {
+      a = (double)(x[i] * (g[i] * c[i]));
+      b = (double)(xo * (go * s[i]));
+    } else if constexpr (A == ACT_F16) {
+      a = (double)x[i] * (double)(g[i] * c[i]);
+      b = (double)xo * (double)(go * s[i]);
+    } else {
+      a = (double)x[i] * ((double)g[i] * (double)c[i]);
+      b = (double)xo * ((double)go * (double)s[i]);
+    }
+    z[i] = (float)(r * (lo ? a - b : a + b));
   }
 }
 
@@ -163,46 +193,60 @@ __device__ __forceinline__ void norm_rope(const float* x, const float* g, const 
 // that each take a head's K and V.
 template <int A>
 __global__ void pkv_append_kernel(PkvRowArgs a) {
-  const int32_t* plan = a.plan;
-  const int row = blockIdx.x;
-  if (row >= min(plan[PH_ROWS], a.rows)) return;
+  const plan_t plan = (plan_t)(uint64_t)a.plan;
+  const int row = blockIdx.x, rows = plan[PH_ROWS];
   const int u = threadIdx.x >> 4, dc = threadIdx.x & 15;
   if (u >= a.nh + a.nkv) return;     // whole 16-lane rows: the shuffles below stay inside one
-  const int s = seq_of(plan + plan[PH_ROW0], plan[PH_NSEQ], row);
-  const int pos = plan[plan[PH_POS0] + s] + row - plan[plan[PH_ROW0] + s];
+  // what the row index alone leads to, before the plan is looked at
   const size_t base = (size_t)row * (a.nh + 2 * a.nkv) * HD + 8 * dc;
-  float x[8], g[8], c[8], sn[8], z[8];
+  float x[8], v[8], g[8], c[8], sn[8], z[8];
   load8<A>(a.x, base + (size_t)u * HD, x);
-  load8<A>(a.cos, (size_t)pos * (HD / 2) + 8 * (dc & 7), c);
-  load8<A>(a.sin, (size_t)pos * (HD / 2) + 8 * (dc & 7), sn);
+  if (u >= a.nh) load8<A>(a.x, base + (size_t)(u + a.nkv) * HD, v);
+  load8<A>(u < a.nh ? a.qn_w : a.kn_w, 8 * dc, g);
+  if (row >= rows) return;
+  const Place p = place_of(a, plan, rows, row);
+  load8<A>(a.cos, (size_t)p.pos * (HD / 2) + 8 * (dc & 7), c);
+  load8<A>(a.sin, (size_t)p.pos * (HD / 2) + 8 * (dc & 7), sn);
   if (u < a.nh) {
-    load8<A>(a.qn_w, 8 * dc, g);
-    norm_rope<float>(x, g, c, sn, dc, a.eps, z);
+    norm_rope_q(x, g, c, sn, dc, a.eps, z);
     store8<A>(a.q_out, ((size_t)row * a.nh + u) * HD + 8 * dc, z);
   } else {
-    float v[8];
-    load8<A>(a.x, base + (size_t)(u + a.nkv) * HD, v);
-    load8<A>(a.kn_w, 8 * dc, g);
-    norm_rope<double>(x, g, c, sn, dc, a.eps, z);
-    store_kv<A>(head_of(plan, s, pos, a.layer, a.nkv, u - a.nh), pos % kPkvPage, dc, z, v);
+    norm_rope_k<A>(x, g, c, sn, dc, a.eps, z);
+    store_kv<A>(p.page + (u - a.nh) * kPkvHeadBytes, p.pos % kPkvPage, dc, z, v);
   }
+}
+
+// The decoder's own tables hold the host's 32-bit cosines, of which one in some
+// thousand is off by its last bit, and one in a million still is after the
+// rounding to bf16.  A bit of a table moves the keys that lie next to a 4-bit
+// border, by a quarter of their value: the append has tables of its own, from
+// 64-bit cosines of the same angles.
+template <int A>
+__global__ void __launch_bounds__(256) pkv_rope_kernel(RopeFreqs f, int positions, void* cos_out, void* sin_out) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (size_t)positions * (HD / 2)) return;
+  const double angle = (double)((float)(i / (HD / 2)) * f.inv[i % (HD / 2)]);
+  // the empty asm keeps the two roundings apart: the compiler makes one of them
+  float c = (float)cos(angle), s = (float)sin(angle);
+  asm volatile("" : "+v"(c), "+v"(s));
+  ((typename ActT<A>::T*)cos_out)[i] = st_act<A>(c);
+  ((typename ActT<A>::T*)sin_out)[i] = st_act<A>(s);
 }
 
 // K and V rows as they are (already rotated) into the plan's positions.
 template <int A>
 __global__ void pkv_write_kernel(PkvRowArgs a) {
-  const int32_t* plan = a.plan;
-  const int row = blockIdx.x;
-  if (row >= min(plan[PH_ROWS], a.rows)) return;
+  const plan_t plan = (plan_t)(uint64_t)a.plan;
+  const int row = blockIdx.x, rows = plan[PH_ROWS];
   const int u = threadIdx.x >> 4, dc = threadIdx.x & 15;
   if (u >= a.nkv) return;
-  const int s = seq_of(plan + plan[PH_ROW0], plan[PH_NSEQ], row);
-  const int pos = plan[plan[PH_POS0] + s] + row - plan[plan[PH_ROW0] + s];
   const size_t at = ((size_t)row * a.nkv + u) * HD + 8 * dc;
   float k[8], v[8];
   load8<A>(a.x, at, k);
   load8<A>(a.v, at, v);
-  store_kv<A>(head_of(plan, s, pos, a.layer, a.nkv, u), pos % kPkvPage, dc, k, v);
+  if (row >= rows) return;
+  const Place p = place_of(a, plan, rows, row);
+  store_kv<A>(p.page + u * kPkvHeadBytes, p.pos % kPkvPage, dc, k, v);
 }
 
 __device__ __forceinline__ void decode8(uint32_t w, int byte, float* o) {
@@ -219,28 +263,31 @@ __device__ __forceinline__ void decode8(uint32_t w, int byte, float* o) {
 // The plan's rows back, as the values they stand for.
 template <int A>
 __global__ void pkv_read_kernel(PkvRowArgs a) {
-  const int32_t* plan = a.plan;
-  const int row = blockIdx.x;
-  if (row >= min(plan[PH_ROWS], a.rows)) return;
+  const plan_t plan = (plan_t)(uint64_t)a.plan;
+  const int row = blockIdx.x, rows = plan[PH_ROWS];
+  if (row >= rows) return;
   const int u = threadIdx.x >> 4, dc = threadIdx.x & 15;
   if (u >= a.nkv) return;
-  const int s = seq_of(plan + plan[PH_ROW0], plan[PH_NSEQ], row);
-  const int pos = plan[plan[PH_POS0] + s] + row - plan[plan[PH_ROW0] + s];
-  const int t = pos % kPkvPage;
-  const uint8_t* head = head_of(plan, s, pos, a.layer, a.nkv, u);
+  const Place p = place_of(a, plan, rows, row);
+  const int t = p.pos % kPkvPage;
+  const gmem_t head = p.page + u * kPkvHeadBytes;
   float k[8], v[8];
-  decode8(*(const uint32_t*)(head + t * 64 + dc * 4), head[kPkvKs + kscale_at(t, dc >> 2)], k);
-  decode8(*(const uint32_t*)(head + kPkvV + t * 64 + dc * 4), head[kPkvVs + 64 * (dc >> 2) + t], v);
+  decode8(*(gmem4_t)(head + t * 64 + dc * 4), head[kPkvKs + kscale_at(t, dc >> 2)], k);
+  decode8(*(gmem4_t)(head + kPkvV + t * 64 + dc * 4), head[kPkvVs + 64 * (dc >> 2) + t], v);
   const size_t at = ((size_t)row * a.nkv + u) * HD + 8 * dc;
   if (a.k_out) store8<A>(a.k_out, at, k);
   if (a.v_out) store8<A>(a.v_out, at, v);
 }
 
-constexpr int kCopyUnroll = 4;
+constexpr int kCopyUnroll = 4, kFewPairs = 16;
+struct FewPairs {
+  int32_t src[kFewPairs], dst[kFewPairs];
+};
 
 // A page of a layer is contiguous: pairs x layers pieces of nkv * 544 16-byte
 // words, all of them one index range.
-__global__ void __launch_bounds__(256) pkv_copy_kernel(PkvPairs p, int n, uint32_t layers,
+template <class PAIRS>
+__global__ void __launch_bounds__(256) pkv_copy_kernel(PAIRS p, int n, uint32_t layers,
                                                        uint32_t words, const u32x4* src, int src_pages, u32x4* dst,
                                                        int dst_pages) {
   const uint32_t total = (uint32_t)n * layers * words;   // below 2^31 (launch_pkv_copy)
@@ -276,6 +323,14 @@ __global__ void pkv_clear_plan_kernel(int32_t* plan) {
     return hipGetLastError();                                                                      \
   } while (0)
 
+hipError_t launch_pkv_rope(int act, const RopeFreqs& f, int positions, void* cos, void* sin, hipStream_t s) {
+  const dim3 grid((unsigned)(((size_t)positions * (HD / 2) + 255) / 256)), block(256);
+  if (act == ACT_F32) hipLaunchKernelGGL(pkv_rope_kernel<ACT_F32>, grid, block, 0, s, f, positions, cos, sin);
+  else if (act == ACT_F16) hipLaunchKernelGGL(pkv_rope_kernel<ACT_F16>, grid, block, 0, s, f, positions, cos, sin);
+  else hipLaunchKernelGGL(pkv_rope_kernel<ACT_BF16>, grid, block, 0, s, f, positions, cos, sin);
+  return hipGetLastError();
+}
+
 hipError_t launch_pkv_append(int act, const PkvRowArgs& a, hipStream_t s) {
   BY_ACT(pkv_append_kernel, 16 * (a.nh + a.nkv));
 }
@@ -291,8 +346,20 @@ hipError_t launch_pkv_copy(const PkvPairs& p, int n, int layers, int nkv, const 
   const int words = nkv * (kPkvHeadBytes / 16);
   const int64_t per = 256 * kCopyUnroll, groups = ((int64_t)n * layers * words + per - 1) / per;
   if (n < 1 || n > kPkvPairs || (int64_t)n * layers * words > INT32_MAX - 2 * per) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(pkv_copy_kernel, dim3((unsigned)groups), dim3(256), 0, s, p, n, layers, words,
-                     (const u32x4*)src_pool, src_pages, (u32x4*)dst_pool, dst_pages);
+  const dim3 grid((unsigned)groups), block(256);
+  if (n <= kFewPairs) {
+    // few pairs: fewer bytes of kernel arguments to write for the launch
+    FewPairs f;
+    for (int i = 0; i < n; ++i) {
+      f.src[i] = p.src[i];
+      f.dst[i] = p.dst[i];
+    }
+    hipLaunchKernelGGL(pkv_copy_kernel<FewPairs>, grid, block, 0, s, f, n, layers, words,
+                       (const u32x4*)src_pool, src_pages, (u32x4*)dst_pool, dst_pages);
+  } else {
+    hipLaunchKernelGGL(pkv_copy_kernel<PkvPairs>, grid, block, 0, s, p, n, layers, words,
+                       (const u32x4*)src_pool, src_pages, (u32x4*)dst_pool, dst_pages);
+  }
   return hipGetLastError();
 }
 

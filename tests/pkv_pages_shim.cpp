@@ -2,7 +2,7 @@
 #include "pkv_pages.h"
 
 static PkvPages::Copies g_copies;
-static std::vector<int32_t> g_plan, g_to;
+static std::vector<int32_t> g_plan, g_far, g_to;
 
 extern "C" {
 void* pages_new(int pages, int seqs, int rows, int max_len, int window, int sinks) {
@@ -40,15 +40,20 @@ const int32_t* pages_of(void* p, int s) { return ((PkvPages*)p)->seqs[s].pages.d
 const int32_t* pages_refs(void* p) { return ((PkvPages*)p)->refs.data(); }
 int pages_free_n(void* p) { return ((PkvPages*)p)->free_pages(); }
 int pages_plan(void* p, int nkv, int tile, int n, const int32_t* seqs, const int32_t* counts) {
-  g_plan = pkv_build_plan(*(PkvPages*)p, nkv, tile, n, seqs, counts);
+  g_plan = pkv_build_plan(*(PkvPages*)p, nkv, tile, n, seqs, counts, &g_far);
   return (int)g_plan.size();
 }
 const int32_t* plan_words() { return g_plan.data(); }
+int plan_far(const int32_t** out) {
+  *out = g_far.data();
+  return (int)g_far.size();
+}
 void plan_bounds(int nkv, int seqs, int rows, int max_len, int tile, int64_t* out) {
   const PkvBounds b = pkv_bounds(nkv, seqs, rows, max_len, tile);
   out[0] = b.dec_items;
   out[1] = b.tiles;
   out[2] = b.pre_slots;
-  out[3] = (int64_t)b.words;
+  out[3] = (int64_t)b.rows_at;
+  out[4] = (int64_t)b.words;
 }
 }

@@ -1,13 +1,13 @@
 """The paged 4-bit KV cache on the device against tests/pkv_ref.py.
 
 Tolerances.  u is half a unit in the last place of the output's type relative to
-the value (f32 2^-24, bf16 2^-8 of the power of two below, so 2^-8 relative at
-most; f16 2^-11).  K and V come back exactly.  q: one rounding, after f32
+the value: f32 2^-24, f16 2^-11, bf16 2^-8.  K and V come back exactly.  q: one rounding, after f32
 arithmetic whose relative error (a sum of 128 squares, a root, a division, three
 products and a sum) stays under 32 * 2^-24 of the rotated pair's length.
-Context: p and the sums are f32; p meets V as 16 bits in decode rows of 16-bit
-caches, as 8 (bf16) or 11 (f16) in many-token rows, as 24 in f32 caches.  With
-every p off by at most the factor r = 2^-17, 2^-9, 2^-12 or 2^-24, and l with it, a
+Context: p and the sums are f32; p meets V as a sum of two bf16 terms in decode
+rows of 16-bit caches, as one bf16 or f16 value in many-token rows, as three bf16
+terms in f32 caches.  With every p off by at most the factor r = 2^-16 (2^-8 of
+what the first term left), 2^-8, 2^-11 or 2^-24, and l with it, a
 context element moves by at most 2 r max|v|.  A score is a sum of 128 products
 in four MFMAs (f32 caches: twelve) of 32: at most 9 (17) roundings on a path,
 each 2^-24 of at most sum|q k| / sqrt(128) < 30 here, then the exponent's own
@@ -64,7 +64,7 @@ def fill(cache, layer, seqs, kv):
 
 
 def ctx_bound(prec, want, vmax, decode):
-    r = {"bf16": 2.0 ** -17 if decode else 2.0 ** -9, "f16": 2.0 ** -17 if decode else 2.0 ** -12,
+    r = {"bf16": 2.0 ** -16 if decode else 2.0 ** -8, "f16": 2.0 ** -16 if decode else 2.0 ** -11,
          "f32": 2.0 ** -24}[prec]
     return (2 * r + 2.0 ** -14) * vmax + U[prec] * np.abs(want) + 1e-30
 

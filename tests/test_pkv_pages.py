@@ -11,8 +11,7 @@ import numpy as np
 import pytest
 
 ROOT = Path(__file__).resolve().parents[1]
-HDR = dict(ROWS=0, NSEQ=1, PAGES=4, NDEC=5, WORK=6, NWORK=7, NSPLIT=8, ROW0=9, POS0=10, TOFF=11,
-           PITEM=13, SPLIT=14, WORDS=32)
+HDR = dict(ROWS=0, PAGES=3, NDEC=4, NWORK=5, NSPLIT=6, WORK=7, PITEM=8, SPLIT=9, WORDS=32, ITEMS=32 + 512)
 P = 64
 
 
@@ -30,7 +29,7 @@ def shim(tmp_path_factory):
                             ("pages_extend", I, [V, I, PI, PI]), ("pages_compact", I, [V, I, I]), ("copies_n", I, []),
                             ("copies_src", PI, []), ("copies_dst", PI, []), ("pages_len", I, [V, I]),
                             ("pages_n", I, [V, I]), ("pages_of", PI, [V, I]), ("pages_refs", PI, [V]),
-                            ("pages_free_n", I, [V]), ("pages_plan", I, [V, I, I, I, PI, PI]), ("plan_words", PI, []),
+                            ("pages_free_n", I, [V]), ("pages_plan", I, [V, I, I, I, PI, PI]), ("plan_words", PI, []), ("plan_far", I, [ctypes.POINTER(PI)]),
                             ("plan_bounds", None, [I] * 5 + [ctypes.POINTER(ctypes.c_int64)])):
         fn = getattr(h, name)
         fn.restype, fn.argtypes = res, args
@@ -270,28 +269,28 @@ def test_plans_cover_what_each_row_sees_once(shim, seed):
                 left -= m
         assert shim.pages_extend(c.p, n_seqs, arr(seqs), arr(counts)) == 0
         w = _plan(c, nkv, tile, seqs, counts)
-        b = (ctypes.c_int64 * 4)()
+        b = (ctypes.c_int64 * 5)()
         shim.plan_bounds(nkv, n_seqs, max_rows, max_len, tile, b)
         assert len(w) <= b[3] and w[HDR["NDEC"]] <= b[0]
         rows = sum(counts)
-        assert w[HDR["ROWS"]] == rows and w[HDR["NSEQ"]] == n_seqs
-        row0 = w[w[HDR["ROW0"]]:][: n_seqs + 1]
-        assert row0.tolist() == np.concatenate([[0], np.cumsum(counts)]).tolist()
-        assert w[w[HDR["POS0"]]:][:n_seqs].tolist() == lens
-        toff = w[w[HDR["TOFF"]]:][:n_seqs]
-        seq_at = {}
-        for i in range(n_seqs):
-            if counts[i]:
-                t = shim.pages_of(c.p, seqs[i])[: shim.pages_n(c.p, seqs[i])]
-                assert w[toff[i]:toff[i] + len(t)].tolist() == t
-                for k in range(counts[i]):
-                    seq_at[int(row0[i]) + k] = i
+        assert w[HDR["ROWS"]] == rows
+        row0 = np.concatenate([[0], np.cumsum(counts)])
+        seq_at = {int(row0[i]) + k: i for i in range(n_seqs) for k in range(counts[i])}
+        far = ctypes.POINTER(ctypes.c_int32)()
+        n_far = shim.plan_far(ctypes.byref(far))
+        assert n_far == (2 * rows if rows > 256 else 0) and b[3] + n_far <= b[4]
+        at = np.array(far[:n_far] if n_far else w[HDR["WORDS"]:][: 2 * rows]).reshape(-1, 2)
+        tables = [shim.pages_of(c.p, s)[: shim.pages_n(c.p, s)] for s in seqs]
+        for row, (pos, page) in enumerate(at.tolist()):
+            i = seq_at[row]
+            assert pos == lens[i] + row - row0[i] and page == tables[i][pos // P]
         seen_pages = {row: [] for row in range(rows)}
         slots = {}
 
         def walk(row, pos, n, table, sp, wp, v0, v1, slot):
             i = seq_at[row]
-            assert table == toff[i] and pos == lens[i] + row - row0[i] and 0 <= v0 < v1
+            assert w[table:table + len(tables[i])].tolist() == tables[i]
+            assert pos == lens[i] + row - row0[i] and 0 <= v0 < v1
             pages = [v if v < sp else wp + v - sp for v in range(v0, v1)]
             for pg in pages:
                 assert w[table + pg] >= 0, "an item names a released page"
@@ -300,9 +299,12 @@ def test_plans_cover_what_each_row_sees_once(shim, seed):
                 seen_pages[row + k] += pages
             return slot
 
-        dec = w[HDR["WORDS"]:][: 12 * w[HDR["NDEC"]]].reshape(-1, 12)
-        for row, pos, table, sp, wp, v0, v1, slot, first, parts, *_ in dec.tolist():
+        dec = w[HDR["ITEMS"]:][: 16 * w[HDR["NDEC"]]].reshape(-1, 16)
+        for row, pos, table, sp, wp, v0, v1, slot, first, parts, *ids in dec.tolist():
             walk(row, pos, 1, table, sp, wp, v0, v1, slot)
+            for j in range(4):
+                v = min(v0 + j, v1 - 1)
+                assert ids[j] == w[table + (v if v < sp else wp + v - sp)]
             assert first <= slot < first + parts and slot < b[0] and slot not in slots
             slots[slot] = (row, first, parts)
         for slot, (row, first, parts) in slots.items():
