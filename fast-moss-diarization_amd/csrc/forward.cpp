@@ -1388,6 +1388,10 @@ extern "C" int fmd_dec_logprobs(fmd_dec* d, int n, const uint32_t* tokens, int t
   for (int i = 0; tokens && i < n; ++i)
     if (tokens[i] >= (uint32_t)d->V) return fmd_fail(FMD_ERR_ARG, "token id out of range");
   HIPCHK(hipSetDevice(d->device));
+  hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+  HIPCHK(hipStreamIsCapturing(d->stream, &cap));
+  if (cap != hipStreamCaptureStatusNone)
+    return fmd_fail(FMD_ERR_STATE, "host results cannot be captured: use fmd_op_logprobs");
   LogprobArgs a;
   CHK(logprob_args(d, d->ws.logits.p, FMD_DT_F32, n, d->V, d->V, top, &a));
   // tokens | logp | entropy | ids | best

@@ -63,10 +63,10 @@ int check_cache(const fmd_pkv* c) {
 // A call on the tables, with its message.
 int told(const fmd_pkv* c, int rc) { return rc ? fmd_fail(rc, c->tab.error) : 0; }
 
-int check_idle(const fmd_pkv* c) {
-  HIPCHK(hipSetDevice(c->dec->device));
+int check_idle(const fmd_dec* d) {
+  HIPCHK(hipSetDevice(d->device));
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-  HIPCHK(hipStreamIsCapturing(c->dec->stream, &cap));
+  HIPCHK(hipStreamIsCapturing(d->stream, &cap));
   if (cap != hipStreamCaptureStatusNone)
     return fmd_fail(FMD_ERR_STATE, "the cache's pages cannot change under graph capture");
   return 0;
@@ -225,7 +225,7 @@ extern "C" int fmd_pkv_create(fmd_dec* d, int pages, int max_seqs, int max_rows,
     return fmd_fail(FMD_ERR_ARG, "max_seqs above 65536 or max_rows above 1048576");
   if (window < 0 || sinks < 0) return fmd_fail(FMD_ERR_ARG, "negative window or sinks");
   if (!window && sinks) return fmd_fail(FMD_ERR_ARG, "sinks need a window");
-  HIPCHK(hipSetDevice(d->device));
+  CHK(check_idle(d));
   fmd_pkv* c = nullptr;
   int rc = guarded([&]() {
     c = new fmd_pkv();
@@ -285,7 +285,7 @@ extern "C" int fmd_pkv_fork(fmd_pkv* c, int seq, int32_t* out) {
   CHK(check_cache(c));
   if (!out) return fmd_fail(FMD_ERR_ARG, "null argument");
   CHK(told(c, c->tab.check(seq)));
-  CHK(check_idle(c));
+  CHK(check_idle(c->dec));
   CHK(guarded([&]() { return told(c, c->tab.fork(seq, out)); }));
   return drop_plan(c);   // the planned rows of `seq` would land in pages that are now shared
 }
@@ -294,7 +294,7 @@ extern "C" int fmd_pkv_copy(fmd_pkv* c, int seq, int32_t* out) {
   CHK(check_cache(c));
   if (!out) return fmd_fail(FMD_ERR_ARG, "null argument");
   CHK(told(c, c->tab.check(seq)));
-  CHK(check_idle(c));
+  CHK(check_idle(c->dec));
   return guarded([&]() {
     PkvPages::Copies l;
     int32_t made = -1;
@@ -312,7 +312,7 @@ extern "C" int fmd_pkv_copy(fmd_pkv* c, int seq, int32_t* out) {
 extern "C" int fmd_pkv_free(fmd_pkv* c, int seq) {
   CHK(check_cache(c));
   CHK(told(c, c->tab.check(seq)));
-  CHK(check_idle(c));
+  CHK(check_idle(c->dec));
   CHK(guarded([&]() { return told(c, c->tab.free(seq)); }));
   return drop_plan(c);
 }
@@ -320,7 +320,7 @@ extern "C" int fmd_pkv_free(fmd_pkv* c, int seq) {
 extern "C" int fmd_pkv_truncate(fmd_pkv* c, int seq, int len) {
   CHK(check_cache(c));
   CHK(told(c, c->tab.check(seq)));
-  CHK(check_idle(c));
+  CHK(check_idle(c->dec));
   const int before = c->tab.seqs[seq].len;
   return guarded([&]() {
     CHK(told(c, c->tab.truncate(seq, len)));
@@ -330,7 +330,7 @@ extern "C" int fmd_pkv_truncate(fmd_pkv* c, int seq, int len) {
 
 extern "C" int fmd_pkv_resize(fmd_pkv* c, int pages) {
   CHK(check_cache(c));
-  CHK(check_idle(c));
+  CHK(check_idle(c->dec));
   return guarded([&]() {
     const bool in_place = pages == c->tab.pages;
     std::vector<int32_t> to;
@@ -381,7 +381,7 @@ extern "C" int fmd_pkv_pool(const fmd_pkv* c, void** data, size_t* bytes) {
 
 extern "C" int fmd_pkv_plan(fmd_pkv* c, int n, const int32_t* seqs, const int32_t* counts) {
   CHK(check_cache(c));
-  CHK(check_idle(c));
+  CHK(check_idle(c->dec));
   return guarded([&]() {
     fmd_dec* d = c->dec;
     PkvPages::Copies l;

@@ -392,6 +392,7 @@ class Qwen3:
         self.precision = Precision.parse(precision) if isinstance(precision, str) else Precision(precision)
         # engine.rs:239-243: the RoPE table covers min(max_position_embeddings, 65536).
         self.max_len = max_len or min(cfg.max_position_embeddings, 65_536)
+        self.device = device
         h = ctypes.c_void_p()
         c = cfg.to_c()
         _check(lib().fmd_dec_create(ctypes.byref(c), int(self.precision), device, self.max_len,

@@ -114,7 +114,7 @@ class PagedKvCache:
         _check(lib().fmd_pkv_pool(self.handle, ctypes.byref(ptr), ctypes.byref(size)))
         layers = self.model.cfg.num_hidden_layers
         shape = (layers, self.num_pages, size.value // (layers * self.num_pages))
-        return torch.as_tensor(_Pool(self, ptr.value, shape), device="cuda")
+        return torch.as_tensor(_Pool(self, ptr.value, shape), device=torch.device("cuda", self.model.device))
 
     # -- a plan and what runs on it (device pointers) --------------------------
     def plan(self, seqs: Sequence[int], counts: Sequence[int]) -> None:
@@ -179,12 +179,23 @@ class PagedKvCache:
                                   None if keep is None else _data_ptr(keep), on_dev, _ptr(out)))
         return out
 
-    def prefill(self, seq: int, tokens: Sequence[int], chunk: int | None = None) -> None:
-        """``step`` over a prompt in pieces of at most `chunk` (default max_rows)
-        tokens; under a window, pages that fall behind it are reused in between."""
-        size = min(chunk or self.max_rows, self.max_rows)
-        for at in range(0, len(tokens), size):
-            self.step([seq], [tokens[at:at + size]], logits=False)
+    def prefill(self, seqs: Sequence[int], prompts: Sequence[Sequence[int]]) -> None:
+        """``step`` over prompts of any length, as many tokens at a time as the
+        cache takes; under a window, pages that fall behind it are reused in
+        between."""
+        at = [0] * len(prompts)
+        while True:
+            room, which, pieces = self.max_rows, [], []
+            for i, p in enumerate(prompts):
+                piece = p[at[i]:at[i] + room]
+                if len(piece):
+                    which.append(seqs[i])
+                    pieces.append(piece)
+                    at[i] += len(piece)
+                    room -= len(piece)
+            if not which:
+                return
+            self.step(which, pieces, logits=False)
 
 
 @dataclass
@@ -216,11 +227,9 @@ def generate_paged(cache: PagedKvCache, prompts: Sequence[Sequence[int]], budget
         for _ in prompts:
             seqs.append(cache.open())
         live = list(range(len(prompts)))
-        feed = []
-        for i in live:
-            # all but the last token, so that the first step has every row's logits
-            cache.prefill(seqs[i], list(prompts[i][:-1]))
-            feed.append([prompts[i][-1]])
+        # all but the last tokens, so that the first step has every row's logits
+        cache.prefill(seqs, [list(p[:-1]) for p in prompts])
+        feed = [[p[-1]] for p in prompts]
         for step in range(budget):
             if not live:
                 break

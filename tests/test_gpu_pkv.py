@@ -233,6 +233,41 @@ def test_long_row_in_many_items(fmd):
     run_attention(fmd, "bf16", 2, [4096], [90], nkv=1)
 
 
+def test_more_rows_than_work_group_slots(fmd):
+    """300 sequences: each row is an item of its own, in several rounds."""
+    run_attention(fmd, "bf16", 1, [1 + (7 * i) % 200 for i in range(300)], [1] * 300)
+
+
+def test_large_plans(fmd):
+    """More new tokens than the plan's first upload holds, mixed with decode rows."""
+    run_attention(fmd, "f16", 2, [700, 300, 1, 513], [600, 1, 1, 513])
+
+
+def test_queries_with_nan_stay_in_their_rows(fmd):
+    m, cfg, _ = make(fmd, "bf16")
+    c = fmd.PagedKvCache(m, pages=8, max_seqs=2, max_rows=128)
+    s = [c.open(), c.open()]
+    kv = [(randn((n, 2, 128), torch.bfloat16, n), randn((n, 2, 128), torch.bfloat16, n + 1)) for n in (100, 60)]
+    fill(c, 0, s, [(k[:-n], v[:-n]) for (k, v), n in zip(kv, (1, 33))])
+    c.plan(s, [1, 33])
+    a, b = (up(torch.cat([kv[0][j][-1:], kv[1][j][-33:]])) for j in (0, 1))
+    c.write(0, a.data_ptr(), b.data_ptr())
+    q = randn((34, 4, 128), torch.bfloat16, 5)
+    out = up(torch.zeros((34, 4, 128), dtype=torch.bfloat16))
+    ref_out = up(torch.zeros((34, 4, 128), dtype=torch.bfloat16))
+    qd = up(q)
+    c.attention(0, qd.data_ptr(), ref_out.data_ptr())
+    q[0, 1, 7], q[9, 2, 0] = float("nan"), float("inf")
+    qd = up(q)
+    c.attention(0, qd.data_ptr(), out.data_ptr())
+    torch.cuda.synchronize()
+    got, want = out.cpu(), ref_out.cpu()
+    bad = torch.zeros((34, 4), dtype=torch.bool)
+    bad[0, 1] = bad[9, 2] = True
+    assert got[bad].isnan().any(-1).all()
+    assert torch.equal(got[~bad], want[~bad])
+
+
 def test_nan_and_infinity_stay_where_they_are_seen(fmd):
     """A token with a NaN or an infinity in K or V poisons its head's contexts
     that see it, and no other, in decode and many-token rows."""

@@ -333,3 +333,25 @@ def test_plans_cover_what_each_row_sees_once(shim, seed):
             assert need <= set(seen_pages[row]), (row, p)
     finally:
         shim.pages_delete(c.p)
+
+
+def test_entry_points_refuse_null_handles_without_a_device(fmd):
+    lib, n = fmd.lib(), ctypes.c_int32()
+    h, p, z = ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_size_t()
+    calls = [lambda: lib.fmd_pkv_create(None, 1, 1, 1, 0, 0, ctypes.byref(h)), lambda: lib.fmd_pkv_open(None, ctypes.byref(n)),
+             lambda: lib.fmd_pkv_fork(None, 0, ctypes.byref(n)), lambda: lib.fmd_pkv_copy(None, 0, ctypes.byref(n)),
+             lambda: lib.fmd_pkv_free(None, 0), lambda: lib.fmd_pkv_truncate(None, 0, 0),
+             lambda: lib.fmd_pkv_resize(None, 1), lambda: lib.fmd_pkv_len(None, 0), lambda: lib.fmd_pkv_free_pages(None),
+             lambda: lib.fmd_pkv_pages(None, 0, None, 0, ctypes.byref(n)),
+             lambda: lib.fmd_pkv_pool(None, ctypes.byref(p), ctypes.byref(z)), lambda: lib.fmd_pkv_plan(None, 0, None, None),
+             lambda: lib.fmd_op_pkv_append(None, None, 0, None, None), lambda: lib.fmd_op_pkv_write(None, None, 0, None, None),
+             lambda: lib.fmd_op_pkv_read(None, None, 0, None, None),
+             lambda: lib.fmd_op_pkv_attention(None, None, 0, None, None),
+             lambda: lib.fmd_op_pkv_copy_pages(None, 0, None, None),
+             lambda: lib.fmd_dec_step(None, None, 1, None, None, None, None, 0, None),
+             lambda: lib.fmd_op_logprobs(None, None, 0, 1, 1, 1, None, 0, None, None, None, None),
+             lambda: lib.fmd_dec_logprobs(None, 1, None, 0, None, None, None, None)]
+    for i, call in enumerate(calls):
+        assert call() == -1, i
+    assert lib.fmd_pkv_destroy(None) == 0
+    assert lib.fmd_pkv_bytes(None, 5) == 0
