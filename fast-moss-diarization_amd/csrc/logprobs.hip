@@ -16,8 +16,8 @@
 // tournament of 15 comparisons finds the largest value; its 15 losers each cost
 // one exponential, so that the largest is left out of S without a test per
 // value.  A wave keeps the alternatives it has seen in its first lanes, in
-// order; only values above the last of them are looked at one by one, which
-// after the first tiles is rare.  Rows are cut so that a launch has about
+// order; only values that can still be among the row's best, by what the
+// work-group's waves have told each other, are looked at one by one.  Rows are cut so that a launch has about
 // kGroups work-groups; the last piece of a row to end joins them all.
 //
 // Alternatives are ordered by value, equal ones by index (lower first, -0 and 0
@@ -90,6 +90,7 @@ __device__ __forceinline__ uint64_t get(const uint64_t* p) {
 
 struct Shared {
   uint64_t joined[kMaxTop];
+  uint32_t told[kWaves];
   uint64_t wave[2][kWaves];
   Stat stat[kWaves];
   uint32_t ticket;
@@ -272,7 +273,7 @@ __device__ __forceinline__ void finish(const LogprobArgs& a, const Shared& sh, S
 }
 
 template <int DT>
-__global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int splits, int per) {
+__global__ void __launch_bounds__(kThreads) __attribute__((amdgpu_num_sgpr(96))) logprob_kernel(LogprobArgs a, int splits, int per) {
   __shared__ Shared sh;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int split = blockIdx.x % splits, row = blockIdx.x / splits;
@@ -288,38 +289,32 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int sp
   }
   Stat st = {-INFINITY, 0.f, 0.f};
   List list = {0, 0};
-  Raw<DT> next;
-  if (t0 < t1) next.load(x, t0 * kTile, a.vocab, lane);
-  for (int t = t0; t < t1; t += kWaves) {
-    const Raw<DT> raw = next;
-    if (t + kWaves < t1) next.load(x, (t + kWaves) * kTile, a.vocab, lane);
-    float v[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) v[e] = raw.get(e);
-    const float tm = add_tile(st, v);
-    if (a.top == 0) continue;
-    // Tiles come in index order, so that a later value has to be above the
-    // list's last (a NaN there, or none, is below all).
-    float floor = list.last ? key_value(list.last) : NAN;
-    if (!__any(!(tm <= floor))) continue;
-    if (list.last == 0) {
-      // A first bound: the top-th largest of the lanes' largest values, with as
-      // many values at or above it.
-      uint32_t b = (uint32_t)(rank_key(tm, 0) >> 32), kth = 0;
-      for (int n = 0; n < a.top; ++n) {
-        kth = wave_max_u32(b);
-        const uint64_t who = __ballot(b == kth);
-        if (lane == __ffsll((long long)who) - 1) b = 0;
-      }
-      // one value below it (-0 has no key of its own): what is not below the bound
-      // is above that
-      if (kth > 2) floor = key_value((uint64_t)(kth - (kth == 0x80000000u ? 2 : 1)) << 32);
-    }
+  // The work-group's common bound: when each of n waves has k values at or above
+  // x and n k >= top, nothing below x is among the row's top.  A wave tells its
+  // k-th value (as the order's upper half); the bound is the least told.
+  const int active = max(1, min(kWaves, t1 - split * per)), k_own = (a.top + active - 1) / active;
+  uint32_t told = 0;
+  float common = NAN;   // NaN: no bound yet
+  auto look = [&]() {
+    uint32_t b = ~0u;
+    // one lane a wave's word; absent waves' words are never the least
+    if (lane < kWaves) b = __hip_atomic_load(&sh.told[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    b = ~wave_max_u32(~b);
+    common = b ? key_value((uint64_t)b << 32) : NAN;
+  };
+  // Candidates: values at or above the common bound, and above the wave's last one
+  // of the tiles before (whose indices are lower: an equal later one loses); any,
+  // NaN too, as long as there is no bound.
+  auto collect = [&](const Raw<DT>& raw, int t, float tm) {
+    const float own = list.last ? key_value(list.last) : NAN;
+    auto open = [&](float f) { return !(f < common) & !(f <= own); };
+    if (!__any(open(tm))) return;
+    look();
+    if (!__any(open(tm))) return;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
       const float f = raw.get(e);
-      const int i = t * kTile + Raw<DT>::index(e, lane);
-      uint64_t who = __ballot(!(f <= floor) && i < a.vocab);
+      uint64_t who = __ballot(open(f) & (t * kTile + Raw<DT>::index(e, lane) < a.vocab));
       while (who) {
         const int l = __ffsll((long long)who) - 1;
         who &= who - 1;
@@ -328,6 +323,44 @@ __global__ void __launch_bounds__(kThreads) logprob_kernel(LogprobArgs a, int sp
         if (k > list.last) list.insert(k, a.top, lane);
       }
     }
+    const uint32_t now = (uint32_t)(lane_u64(list.mine, k_own - 1) >> 32);
+    if (now > told) {
+      told = now;
+      if (lane == 0) __hip_atomic_store(&sh.told[w], now, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    }
+  };
+  Raw<DT> next;
+  auto take = [&](int t, Raw<DT>& raw) {
+    raw = next;
+    if (t + kWaves < t1) next.load(x, (t + kWaves) * kTile, a.vocab, lane);
+    float v[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) v[e] = raw.get(e);
+    return add_tile(st, v);
+  };
+  Raw<DT> raw;
+  float tm = -INFINITY;
+  if (t0 < t1) {
+    next.load(x, t0 * kTile, a.vocab, lane);
+    tm = take(t0, raw);
+  }
+  if (a.top > 0) {
+    // what the waves can tell from their first tiles: the k-th largest of the
+    // lanes' largest values
+    uint32_t b = t0 < t1 ? (uint32_t)(rank_key(tm, 0) >> 32) : 0;
+    for (int n = 0; n < k_own; ++n) {
+      told = wave_max_u32(b);
+      const uint64_t who = __ballot(b == told);
+      if (lane == __ffsll((long long)who) - 1) b = 0;
+    }
+    if (lane == 0) sh.told[w] = t0 < t1 ? told : ~0u;
+    __syncthreads();
+    look();
+    if (t0 < t1) collect(raw, t0, tm);
+  }
+  for (int t = t0 + kWaves; t < t1; t += kWaves) {
+    tm = take(t, raw);
+    if (a.top > 0) collect(raw, t, tm);
   }
   if (lane < a.top) sh.all[w * a.top + lane] = list.mine;
   st = group_join(sh, st);
