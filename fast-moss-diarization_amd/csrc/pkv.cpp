@@ -85,10 +85,8 @@ int drop_plan(fmd_pkv* c) {
 int copy_pairs(fmd_pkv* c, const PkvPages::Copies& l, const void* from, int from_pages, void* to,
                int to_pages) {
   fmd_dec* d = c->dec;
-  // a launch's 16-byte words are counted in 31 bits
-  const int64_t words = (int64_t)d->L * d->nkv * (kPkvHeadBytes / 16);
-  const size_t most = (size_t)std::min<int64_t>(kPkvPairs, ((int64_t)INT32_MAX - 8192) / words);
-  if (most == 0) return fmd_fail(FMD_ERR_ARG, "a page of all layers is too large to copy");
+  const size_t most = (size_t)std::min(kPkvPairs, 65535 / d->L);   // pairs x layers: the grid's second axis
+  if (most == 0) return fmd_fail(FMD_ERR_ARG, "too many layers to copy pages of");
   PkvPairs p;
   for (size_t i = 0; i < l.src.size(); i += most) {
     const size_t n = std::min(most, l.src.size() - i);

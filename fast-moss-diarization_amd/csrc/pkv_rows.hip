@@ -284,28 +284,24 @@ struct FewPairs {
   int32_t src[kFewPairs], dst[kFewPairs];
 };
 
-// A page of a layer is contiguous: pairs x layers pieces of nkv * 544 16-byte
-// words, all of them one index range.
+// A page of a layer is contiguous, nkv * 544 16-byte words: work-groups (x) by
+// layer and pair (y), every thread with its words in flight together.
 template <class PAIRS>
-__global__ void __launch_bounds__(256) pkv_copy_kernel(PAIRS p, int n, uint32_t layers,
-                                                       uint32_t words, const u32x4* src, int src_pages, u32x4* dst,
-                                                       int dst_pages) {
-  const uint32_t total = (uint32_t)n * layers * words;   // below 2^31 (launch_pkv_copy)
-  const uint32_t at = blockIdx.x * (kCopyUnroll * 256) + threadIdx.x;
-  u32x4 w[kCopyUnroll];
-  size_t to[kCopyUnroll];
+__global__ void __launch_bounds__(256) pkv_copy_kernel(PAIRS p, int layers, int words, const u32x4* src,
+                                                       int src_pages, u32x4* dst, int dst_pages) {
+  const int pair = blockIdx.y / layers, layer = blockIdx.y - pair * layers;
+  const int at = blockIdx.x * (256 * kCopyUnroll) + threadIdx.x;
+  const u32x4* from = src + ((size_t)layer * src_pages + p.src[pair]) * words;
+  u32x4* to = dst + ((size_t)layer * dst_pages + p.dst[pair]) * words;
+  if ((int)(blockIdx.x + 1) * (256 * kCopyUnroll) <= words) {
+    u32x4 w[kCopyUnroll];
 #pragma unroll
-  for (int i = 0; i < kCopyUnroll; ++i) {
-    const uint32_t id = at + i * 256;
-    if (id >= total) continue;
-    const uint32_t piece = id / words, off = id - piece * words;
-    const uint32_t pair = piece / layers, layer = piece - pair * layers;
-    w[i] = src[((size_t)layer * src_pages + p.src[pair]) * words + off];
-    to[i] = ((size_t)layer * dst_pages + p.dst[pair]) * words + off;
+    for (int i = 0; i < kCopyUnroll; ++i) w[i] = from[at + i * 256];
+#pragma unroll
+    for (int i = 0; i < kCopyUnroll; ++i) to[at + i * 256] = w[i];
+  } else {
+    for (int i = at; i < words; i += 256) to[i] = from[i];
   }
-#pragma unroll
-  for (int i = 0; i < kCopyUnroll; ++i)
-    if (at + i * 256 < total) dst[to[i]] = w[i];
 }
 
 __global__ void pkv_clear_plan_kernel(int32_t* plan) {
@@ -343,10 +339,9 @@ hipError_t launch_pkv_read(int act, const PkvRowArgs& a, hipStream_t s) {
 
 hipError_t launch_pkv_copy(const PkvPairs& p, int n, int layers, int nkv, const void* src_pool,
                            int src_pages, void* dst_pool, int dst_pages, hipStream_t s) {
-  const int words = nkv * (kPkvHeadBytes / 16);
-  const int64_t per = 256 * kCopyUnroll, groups = ((int64_t)n * layers * words + per - 1) / per;
-  if (n < 1 || n > kPkvPairs || (int64_t)n * layers * words > INT32_MAX - 2 * per) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)groups), block(256);
+  const int words = nkv * (kPkvHeadBytes / 16), per = 256 * kCopyUnroll;
+  if (n < 1 || n > kPkvPairs || (int64_t)n * layers > 65535) return hipErrorInvalidValue;
+  const dim3 grid((words + per - 1) / per, n * layers), block(256);
   if (n <= kFewPairs) {
     // few pairs: fewer bytes of kernel arguments to write for the launch
     FewPairs f;
@@ -354,10 +349,10 @@ hipError_t launch_pkv_copy(const PkvPairs& p, int n, int layers, int nkv, const 
       f.src[i] = p.src[i];
       f.dst[i] = p.dst[i];
     }
-    hipLaunchKernelGGL(pkv_copy_kernel<FewPairs>, grid, block, 0, s, f, n, layers, words,
+    hipLaunchKernelGGL(pkv_copy_kernel<FewPairs>, grid, block, 0, s, f, layers, words,
                        (const u32x4*)src_pool, src_pages, (u32x4*)dst_pool, dst_pages);
   } else {
-    hipLaunchKernelGGL(pkv_copy_kernel<PkvPairs>, grid, block, 0, s, p, n, layers, words,
+    hipLaunchKernelGGL(pkv_copy_kernel<PkvPairs>, grid, block, 0, s, p, layers, words,
                        (const u32x4*)src_pool, src_pages, (u32x4*)dst_pool, dst_pages);
   }
   return hipGetLastError();
