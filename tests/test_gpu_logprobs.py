@@ -134,6 +134,18 @@ def test_row_stride_and_odd_addresses(model):
     check(model, wide[:, 3:4999], "bf16", [0, 1, 2, 3, 4, 4995], 5, ld=5003)
 
 
+def test_rows_beyond_32_bit_offsets(model):
+    """The second row starts 2^31 elements (4 GiB) behind the first."""
+    ld = (1 << 31) + 24
+    buf = torch.empty(ld + 6000, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(8)
+    rows = torch.randn((2, 6000), generator=g).to(torch.bfloat16).cuda()
+    buf[:6000], buf[ld:] = rows[0], rows[1]
+    view = torch.as_strided(buf, (2, 6000), (ld, 1))
+    got, want = scores(model, view, "bf16", [5, 7], 4, ld=ld), scores(model, rows, "bf16", [5, 7], 4)
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
 def test_deterministic_and_on_a_callers_stream(model):
     g = torch.Generator().manual_seed(7)
     x = torch.randn((8, 151936), generator=g).cuda()

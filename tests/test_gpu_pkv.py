@@ -233,6 +233,37 @@ def test_long_row_in_many_items(fmd):
     run_attention(fmd, "bf16", 2, [4096], [90], nkv=1)
 
 
+def test_pages_beyond_4_gib(fmd):
+    """The last pages of a pool whose byte offsets pass 32 bits: the same bits as
+    from a small pool, in decode and many-token rows, and the neighbours' bytes
+    stay as they are."""
+    m, cfg, _ = make(fmd, "bf16", 2, 8, max_len=65536)
+    dt = torch.bfloat16
+    small = fmd.PagedKvCache(m, pages=16, max_seqs=2, max_rows=512)
+    big = fmd.PagedKvCache(m, pages=62 * 1024 + 16, max_seqs=64, max_rows=65536)
+    assert fmd.PagedKvCache.bytes(m, 62 * 1024) > 1 << 32
+    for _ in range(62):
+        big.plan([big.open()], [65536])      # pages taken, nothing written
+    outs = []
+    mark = big.pool()[0, 62 * 1024 - 1]
+    mark.fill_(7)
+    for c in (small, big):
+        s = [c.open(), c.open()]
+        kv = [(randn((n, 8, 128), dt, n), randn((n, 8, 128), dt, n + 1)) for n in (300, 90)]
+        fill(c, 0, s, [(k[:-n], v[:-n]) for (k, v), n in zip(kv, (1, 70))])
+        c.plan(s, [1, 70])
+        a, b = (up(torch.cat([kv[0][j][-1:], kv[1][j][-70:]])) for j in (0, 1))
+        c.write(0, a.data_ptr(), b.data_ptr())
+        q = up(randn((71, 16, 128), dt, 5))
+        out = up(torch.zeros((71, 16, 128), dtype=dt))
+        c.attention(0, q.data_ptr(), out.data_ptr())
+        torch.cuda.synchronize()
+        outs.append(out.cpu())
+    assert min(big.pages(s[0]) + big.pages(s[1])) >= 62 * 1024
+    assert torch.equal(*outs) and outs[0].float().abs().sum() > 0
+    assert (big.pool()[0, 62 * 1024 - 1] == 7).all()
+
+
 def test_more_rows_than_work_group_slots(fmd):
     """300 sequences: each row is an item of its own, in several rounds."""
     run_attention(fmd, "bf16", 1, [1 + (7 * i) % 200 for i in range(300)], [1] * 300)
