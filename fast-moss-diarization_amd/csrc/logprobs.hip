@@ -17,12 +17,14 @@
 // one exponential, so that the largest is left out of S without a test per
 // value.  A wave keeps the alternatives it has seen in its first lanes, in
 // order; only values that can still be among the row's best, by what the
-// work-group's waves have told each other, are looked at one by one.  Rows are cut so that a launch has about
-// kGroups work-groups; the last piece of a row to end joins them all.
-// 1,000 rows of 151,936 bf16 logits (304 MB): 66.5 us, 4.6 TB/s, VALU issue about
+// work-group's waves have told each other, are looked at one by one.  Rows are
+// cut so that a launch has about kGroups work-groups; the last piece of a row to
+// end joins them all.
+// 1,000 rows of 151,936 bf16 logits (304 MB): 65-69 us, 4.6 TB/s, VALU issue about
 // as long; with each wave's list on its own 73, with a search of the work-group
 // for each alternative and a barrier a tile 199.  8 f32 rows: 11.0-13.1 us alone
-// (the chain load -> statistics -> ticket -> join), 4.3 us among others.
+// (the chain load -> statistics -> ticket -> join), among others 4.3-4.7 in some
+// processes and 8.4-8.9 in others.
 //
 // Alternatives are ordered by value, equal ones by index (lower first, -0 and 0
 // are equal), NaN below -inf.
