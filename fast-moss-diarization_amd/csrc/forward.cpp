@@ -160,7 +160,10 @@ int ensure_lane(fmd_dec* d, DecodeLane& w, int B, int cap) {
 int ensure_decode_ws(fmd_dec* d, int B, int cap) {
   Workspace& w = d->ws;
   CHK(w.x.ensure((size_t)B * d->H * d->esz));
-  CHK(w.logits.ensure((size_t)B * d->V * 4));
+  bool moved = false;   // also when the allocation fails: the old buffer is gone
+  const int rc = w.logits.ensure((size_t)B * d->V * 4, &moved);
+  if (moved) d->score_rows = 0;
+  CHK(rc);
   CHK(w.amax.ensure((size_t)gemv_logits_nparts(d->act, d->quant, true, d->H, d->V) * B * 8));
   CHK(ensure_lane(d, w.dec, B, cap));
   CHK(w.ids.ensure((size_t)B * 4));
@@ -551,6 +554,7 @@ int prefill_impl(fmd_dec* d, fmd_kv* kv, const void* emb_dev, const int32_t* pad
   const int fill = d->prefill_rows;
   const int maxM =
       (int)std::min<int64_t>((int64_t)B * total, std::max<int64_t>((int64_t)B * chunk, (int64_t)fill + B));
+  d->score_rows = 0;   // until this call's logits are there
   CHK(ensure_decode_ws(d, std::min(B, kMaxDecodeRows), kv->cap));
   CHK(w.x.ensure((size_t)(maxM + 1) * d->H * d->esz));
   CHK(w.xn.ensure((size_t)maxM * std::max(d->H, d->I) * d->esz));
@@ -926,17 +930,19 @@ extern "C" int fmd_dec_decode_step(fmd_dec* d, fmd_kv* kv, const uint32_t* ids, 
     if (ids[b] >= (uint32_t)d->V) return fmd_fail(FMD_ERR_ARG, "token id out of range");
   CHK(decode_pad_checks(kv, pad, B));
   HIPCHK(hipSetDevice(d->device));
+  d->score_rows = 0;
   CHK(ensure_decode_ws(d, B, kv->cap));
   Workspace& w = d->ws;
   CHK(decode_setup(d, kv, B, pad, ids));
   CHK(decode_layers(d, kv, B, w.pad.as<int32_t>(), nullptr, d->stream));
   kv->len += 1;
   d->logits_rows = B;
-  d->score_rows = B;
   if (logits)
     HIPCHK(hipMemcpyAsync(logits, w.logits.p, (size_t)B * d->V * 4, hipMemcpyDeviceToHost, d->stream));
   HIPCHK(hipStreamSynchronize(d->stream));
-  return check_attn_sync(d);
+  CHK(check_attn_sync(d));
+  d->score_rows = B;
+  return 0;
 }
 
 extern "C" int fmd_dec_generate(fmd_dec* d, const void* embeds, int on_dev, const int32_t* pad,
@@ -1254,6 +1260,7 @@ int paged_forward(fmd_dec* d, fmd_pkv* c, int n, const int32_t* counts, int rows
                   const void* embeds, int on_dev, float* logits) {
   Workspace& w = d->ws;
   hipStream_t s = d->stream;
+  d->logits_rows = d->score_rows = 0;   // until this call's logits are there
   CHK(w.x.ensure((size_t)rows * d->H * d->esz));
   CHK(w.xn.ensure((size_t)rows * std::max(d->H, d->I) * d->esz));
   CHK(w.qkv.ensure((size_t)rows * d->qkvd * d->esz));
@@ -1264,7 +1271,6 @@ int paged_forward(fmd_dec* d, fmd_pkv* c, int n, const int32_t* counts, int rows
   CHK(w.lastrow.ensure((size_t)n * 4));
   CHK(w.logits.ensure((size_t)n * d->V * 4));
   CHK(w.amax.ensure((size_t)gemv_logits_nparts(d->act, d->quant, true, d->H, d->V) * kMaxDecodeRows * 8));
-  d->logits_rows = d->score_rows = 0;
   if (ids) {
     CHK(w.ids.ensure((size_t)rows * 4));
     HIPCHK(hipMemcpyAsync(w.ids.p, ids, (size_t)rows * 4, hipMemcpyHostToDevice, s));

@@ -205,6 +205,26 @@ def test_16_bit_models_follow_the_16_bit_cache(fmd, prec):
         e()
 
 
+def test_scores_end_with_their_logits(fmd):
+    """A call that gives the logits' buffer up for a larger one leaves no logits
+    to score; one that has room for them does."""
+    cfg = tiny_cfg(fmd, layers=1, vocab=64)
+    m = fmd.Qwen3(cfg, "f32", max_len=64).load(fmd.synthetic_weights(cfg, seed=1))
+    c = fmd.PagedKvCache(m, pages=4, max_seqs=2, max_rows=8)
+    s = c.open()
+    want = c.step([s], [[1, 2]]).argmax(-1)
+    x = torch.zeros((4, 256)).cuda()
+    torch.cuda.synchronize()
+    m.op_layer_decode(m.new_caches(1, 8), 0, x.data_ptr(), [0], 1)
+    assert np.array_equal(m.logprobs(1, top=1).top_ids[:, 0], want)
+    m.op_layer_decode(m.new_caches(4, 8), 0, x.data_ptr(), [0] * 4, 4)
+    with pytest.raises(fmd.FmdError, match="no logits"):
+        m.logprobs(1, top=1)
+    want = c.step([s], [[3]]).argmax(-1)
+    m.op_layer_decode(m.new_caches(4, 8), 0, x.data_ptr(), [0] * 4, 4)
+    assert np.array_equal(m.logprobs(1, top=1).top_ids[:, 0], want)
+
+
 def test_failed_steps_leave_the_sequences(fmd, f32):
     m, cfg, w = f32
     c = fmd.PagedKvCache(m, pages=2, max_seqs=2, max_rows=64)
