@@ -39,7 +39,14 @@ constexpr int kThreads = 512, kWaves = kThreads / 64, kPer = 16, kTile = 64 * kP
 constexpr int kGroups = 512;
 constexpr int kMaxTop = 32;
 constexpr int kRanked = 1024;   // keys that a join ranks in LDS
+// Up to this largest value the rounding of m log2e is at most 2^-12, and 2^-err
+// is 1 - err ln2 within (2^-12 ln2)^2 / 2 < 2^-25.
+constexpr float kNear = 4096.f;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Largest and smallest of two, NaN if either is.
+__device__ __forceinline__ float top2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float low2(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 
 // m in the logits' units, s and t over exponents in log2 units (t's as well).
 struct Stat {
@@ -56,15 +63,13 @@ __device__ __forceinline__ Stat join(Stat a, Stat b) {
     a.s += b.s;
     return a;
   }
-  const float d = (b.m - a.m) * kLog2e, f = __builtin_amdgcn_exp2f(d), n = b.s + 1.f;
+  // not below -1000 (2^-1000 is 0, and so is 0 * -1000): the type's lowest value,
+  // as a mask, is further from a logit than the product can say
+  const float d = top2((b.m - a.m) * kLog2e, -1000.f), f = __builtin_amdgcn_exp2f(d), n = b.s + 1.f;
   a.s += f * n;
   a.t += f * (b.t + d * n);
   return a;
 }
-
-// Largest and smallest of two, NaN if either is.
-__device__ __forceinline__ float top2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-__device__ __forceinline__ float low2(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 
 // Order of the alternatives as an integer; 0 is below every value's.
 __device__ __forceinline__ uint64_t rank_key(float v, uint32_t idx) {
@@ -223,9 +228,7 @@ __device__ __forceinline__ float add_tile(Stat& st, float* v) {
       v[i + r] = low2(a, b);
     }
   const float tm = v[0], m = top2(st.m, tm), lo = low2(st.m, tm);
-  // exponents are taken as v log2e - r0; r0's rounding, the same for all of
-  // the tile, is put right in their sums
-  const float mm = m == -INFINITY ? 0.f : m, r0 = mm * kLog2e, err = fmaf(mm, kLog2e, -r0);
+  const float mm = m == -INFINITY ? 0.f : m;
   // the tile's largest value against the running one: the smaller of them
   // loses, with all that was summed below it when that is the running one
   const float d = top2((lo - mm) * kLog2e, -1000.f), f = __builtin_amdgcn_exp2f(d);
@@ -236,14 +239,24 @@ __device__ __forceinline__ float add_tile(Stat& st, float* v) {
     s += st.s;
     t += st.t;
   }
-  float ps = 0.f, pt = 0.f;
-#pragma unroll
-  for (int e = 1; e < kPer; ++e) {
-    // ruled out tokens: 2^-1000 is 0, and so is 0 * -1000
-    const float y = top2(fmaf(v[e], kLog2e, -r0), -1000.f);
+  float ps = 0.f, pt = 0.f, err = 0.f;
+  auto add = [&](float y) {
+    y = top2(y, -1000.f);   // ruled out tokens: 2^-1000 is 0, and so is 0 * -1000
     const float p = __builtin_amdgcn_exp2f(y);
     ps += p;
     pt = fmaf(p, y, pt);
+  };
+  if (__any(!(fabsf(mm) <= kNear))) {
+    // logits so large that r0 below would round by much, or not be finite
+#pragma unroll
+    for (int e = 1; e < kPer; ++e) add((v[e] - mm) * kLog2e);
+  } else {
+    // exponents are taken as v log2e - r0; r0's rounding, the same for all of
+    // the tile, is put right in their sums
+    const float r0 = mm * kLog2e;
+    err = fmaf(mm, kLog2e, -r0);
+#pragma unroll
+    for (int e = 1; e < kPer; ++e) add(fmaf(v[e], kLog2e, -r0));
   }
   const float c = fmaf(-err, kLn2, 1.f);   // 2^-err
   st = {m, fmaf(c, ps, s), fmaf(c, pt - err * ps, t)};

@@ -114,6 +114,33 @@ def test_ruled_out_tokens(model, dtype):
     check(model, x.to(TDT[dtype]).cuda(), dtype, [10, 5000, 0, 10], 4)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_masks_of_the_lowest_value(model, dtype):
+    """Tokens at the type's lowest value: scattered, the row's first or last
+    thousands (whole lanes, waves and pieces), all but one, all (uniform)."""
+    g = torch.Generator().manual_seed(15)
+    low = torch.finfo(TDT[dtype]).min
+    x = torch.randn((6, 150001), generator=g).to(TDT[dtype])
+    x[0, torch.rand(150001, generator=g) < 0.6] = low
+    x[1, :90000] = low
+    x[2, 400:] = low
+    x[3, torch.arange(150001) != 70000] = low
+    x[4] = low
+    x[5, ::2] = -float("inf")
+    x[5, 1::2] = low
+    check(model, x.cuda(), dtype, [int(x[0].float().argmax()), 149999, 3, 70000, 5, 7], 4)
+    check(model, x[:, :1023].contiguous().cuda(), dtype, [0, 1, 2, 3, 4, 5], 4)
+
+
+@pytest.mark.parametrize("at", [4000.0, -5000.0, 1e6, -1e6, 1e30, 3e38, -3e38])
+def test_large_logits(model, at):
+    """Differences of large logits are as good as those of small ones."""
+    g = torch.Generator().manual_seed(16)
+    x = torch.randn((3, 9000), generator=g) * 3 + at
+    check(model, x.cuda(), "f32", [1, 2, 3], 5)
+    check(model, x.to(torch.bfloat16).cuda(), "bf16", [1, 2, 3], 5)
+
+
 def test_rows_without_a_distribution_and_ids_outside(model):
     x = torch.zeros((5, 6000))
     x[0] = -float("inf")
@@ -185,6 +212,38 @@ def test_captured_into_a_graph(model):
             scores(model, x, "f32", [1, 2, 3, 4], 5)     # another call's workspace use
     finally:
         model.set_stream(None)
+
+
+def test_first_call_is_not_captured(fmd):
+    """It allocates; after a call outside a graph the same capture replays."""
+    cfg = fmd.TextConfig(vocab_size=64, hidden_size=256, intermediate_size=256, num_hidden_layers=1,
+                         num_attention_heads=2, num_key_value_heads=2, head_dim=128)
+    m = fmd.Qwen3(cfg, "bf16", max_len=64)
+    st = torch.cuda.Stream()
+    m.set_stream(st.cuda_stream)
+    x, ent = torch.zeros((2, 500)).cuda(), torch.zeros(2).cuda()
+    torch.cuda.synchronize()
+
+    def call():
+        m.op_logprobs(x.data_ptr(), "f32", 2, 500, None, 0, None, ent.data_ptr(), None, None)
+
+    try:
+        with pytest.raises(fmd.FmdError, match="before capturing"):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=st):
+                call()
+        call()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            call()
+        for _ in range(3):
+            ent.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert np.abs(ent.cpu().numpy() - np.log(500)).max() < 1e-5
+    finally:
+        m.set_stream(0)
 
 
 def test_refusals(fmd, model):
