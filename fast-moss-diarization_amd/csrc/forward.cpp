@@ -1256,8 +1256,9 @@ int paged_layers(fmd_dec* d, fmd_pkv* c, int rows) {
   return 0;
 }
 
+// `at` is scratch that outlives the stream's work, as the caller's arrays do.
 int paged_forward(fmd_dec* d, fmd_pkv* c, int n, const int32_t* counts, int rows, const uint32_t* ids,
-                  const void* embeds, int on_dev, float* logits) {
+                  const void* embeds, int on_dev, float* logits, std::vector<int32_t>& at) {
   Workspace& w = d->ws;
   hipStream_t s = d->stream;
   d->logits_rows = d->score_rows = 0;   // until this call's logits are there
@@ -1282,7 +1283,7 @@ int paged_forward(fmd_dec* d, fmd_pkv* c, int n, const int32_t* counts, int rows
   CHK(paged_layers(d, c, rows));
   const void* last = w.x.p;
   if (rows > n) {
-    std::vector<int32_t> at(n);
+    at.resize(n);
     for (int i = 0, r = 0; i < n; ++i) at[i] = (r += counts[i]) - 1;
     HIPCHK(hipMemcpyAsync(w.lastrow.p, at.data(), (size_t)n * 4, hipMemcpyHostToDevice, s));
     LAUNCH(launch_gather_rows(d->act, w.x.p, d->H, w.lastrow.as<int32_t>(), n, d->H, w.lastx.p, d->H, s));
@@ -1349,10 +1350,17 @@ extern "C" int fmd_dec_step(fmd_dec* d, fmd_pkv* c, int n, const int32_t* seqs, 
   for (int64_t i = 0; ids && i < rows; ++i)
     if (ids[i] >= (uint32_t)d->V) return fmd_fail(FMD_ERR_ARG, "token id out of range");
   CHK(fmd_pkv_plan(c, n, seqs, counts));   // refuses more rows than the cache was made for
-  const int rc = paged_forward(d, c, n, counts, (int)rows, ids, embeds, on_dev, logits);
+  std::vector<int32_t> at;
+  int rc;
+  try {
+    rc = paged_forward(d, c, n, counts, (int)rows, ids, embeds, on_dev, logits, at);
+  } catch (const std::exception& e) {
+    rc = fmd_fail(FMD_ERR_OOM, std::string("host: ") + e.what());
+  }
   if (rc) {
-    // the sequences are as long as before
+    // what was queued still reads the host's arrays; the sequences are as long as before
     const std::string keep = fmd_last_error();
+    (void)hipStreamSynchronize(d->stream);
     for (int i = 0; i < n; ++i) (void)fmd_pkv_truncate(c, seqs[i], fmd_pkv_len(c, seqs[i]) - counts[i]);
     return fmd_fail(rc, keep);
   }

@@ -403,7 +403,10 @@ int fmd_dec_step(fmd_dec* dec, fmd_pkv* cache, int n, const int32_t* seqs, const
 
 /* rows x vocab device logits in `dtype`, row stride ld; device targets (rows),
  * logp (rows), entropy (rows), top_ids and top_logp (rows, top).  targets with
- * logp, and entropy, may be NULL; top may be 0. */
+ * logp, and entropy, may be NULL; top may be 0.  Can be captured into a graph
+ * once a call has been made outside one (the first allocates the workspace).
+ * Calls and replays of one decoder share that workspace: run them one after
+ * another. */
 int fmd_op_logprobs(fmd_dec* dec, const void* logits_dev, fmd_dtype dtype, int rows, int vocab,
                     int64_t ld, const int32_t* targets_dev, int top, float* logp_dev,
                     float* entropy_dev, int32_t* top_ids_dev, float* top_logp_dev);
