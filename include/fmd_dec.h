@@ -314,7 +314,8 @@ int fmd_op_logits(fmd_dec* dec, const void* x_dev, int rows, float* logits_dev);
  * to the even code, at most 6.  That is 4.25 bits a value, 136 bytes for a
  * token's K and V of one head and layer.  A token whose K or V of a head holds
  * an infinity or a NaN reads back as NaN in that head, as do the contexts that
- * see it.
+ * see it.  Scores q . k / sqrt(head_dim) may be up to 2^28 in size; contexts of
+ * larger ones can be NaN.
  *
  * Attention is causal.  With window > 0 a query at position p sees the keys
  * j <= p with j > p - window or j < sinks; pages that no later query can see

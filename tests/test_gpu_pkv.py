@@ -264,6 +264,47 @@ def test_pages_beyond_4_gib(fmd):
     assert (big.pool()[0, 62 * 1024 - 1] == 7).all()
 
 
+@pytest.mark.parametrize("prec", ["bf16", "f16", "f32"])
+def test_large_scores(fmd, prec):
+    """One key's score far above the others', up to 2^27 in size: its V alone.
+    The exponent of the largest is then off by half an ulp of 2^28, 8 at most
+    (p and its sum alike)."""
+    dt = TDT[prec]
+    m, cfg, _ = make(fmd, prec, 2, 2)
+    c = fmd.PagedKvCache(m, pages=32, max_seqs=2, max_rows=1024)
+    s = [c.open(), c.open()]
+    big_q, big_k = (1.25 * 2.0 ** 15, 2.0 ** 13) if prec == "f16" else (1.25 * 2.0 ** 20, 2.0 ** 10)
+    lens, counts, top = (900, 700), (1, 130), 5
+    k = [torch.zeros((n, 2, 128), dtype=dt) for n in lens]
+    v = [randn((n, 2, 128), dt, n) for n in lens]
+    for x in k:
+        x[:, :, 0] = big_k / 4
+        x[top, :, 0] = big_k
+    fill(c, 0, s, [(a[:-n], b[:-n]) for a, b, n in zip(k, v, counts)])
+    c.plan(s, counts)
+    a, b = (up(torch.cat([x[i][-n:] for i, n in enumerate(counts)])) for x in (k, v))
+    c.write(0, a.data_ptr(), b.data_ptr())
+    q = torch.zeros((sum(counts), 4, 128), dtype=dt)
+    q[:, :, 0] = big_q
+    q, out = up(q), up(torch.zeros((sum(counts), 4, 128), dtype=dt))
+    c.attention(0, q.data_ptr(), out.data_ptr())
+    torch.cuda.synchronize()
+    got = out.double().cpu().numpy()
+    # V of that key as it is held: written to a sequence of its own and read back
+    c.free(s[0])
+    t = c.open()
+    for i in range(2):
+        one = [up(x[i][top:top + 1].contiguous()) for x in (k, v)]
+        c.plan([t], [1])
+        c.write(0, *(x.data_ptr() for x in one))
+        held = up(torch.zeros((1, 2, 128), dtype=dt))
+        c.read(0, None, held.data_ptr())
+        torch.cuda.synchronize()
+        want = held.double().cpu().numpy()[0].repeat(2, axis=0)
+        rows = got[:1] if i == 0 else got[1:]
+        assert (np.abs(rows - want) <= ctx_bound(prec, want, np.abs(want).max(), i == 0)).all()
+
+
 def test_more_rows_than_work_group_slots(fmd):
     """300 sequences: each row is an item of its own, in several rounds."""
     run_attention(fmd, "bf16", 1, [1 + (7 * i) % 200 for i in range(300)], [1] * 300)
