@@ -481,245 +481,245 @@ __global__ void __launch_bounds__(64 * (PreShape<A, REP>::NW), 2) pkv_prefill_ke
     const int head = unit / n_work;
     const plan_t work = plan + plan[PH_WORK] + unit % n_work;
     for (int it = work[0], end = work[1]; it < end; ++it) {
-    const plan_t ip = plan + plan[PH_PITEM] + it * (int)(sizeof(PkvPreItem) / 4);
-    PkvPreItem item;
-    item.row = ip[0];
-    item.pos = ip[1];
-    item.n = ip[2];
-    item.table = ip[3];
-    item.sp = ip[4];
-    item.wp = ip[5];
-    item.v0 = ip[6];
-    item.v1 = ip[7];
-    item.slot = ip[8];
-    const int rows = min(item.n, a.rows - item.row);
-    if (rows <= 0) continue;
-    const int h = head * REP + r;
-    const plan_t table = plan + item.table;
-    const gmem_t hbase = pool + (size_t)head * kPkvHeadBytes;
-    auto page_of = [&](int v) { return v < item.sp ? v : item.wp + (v - item.sp); };
-    const int last = item.pos + item.n - 1;      // the tile's last position
+      const plan_t ip = plan + plan[PH_PITEM] + it * (int)(sizeof(PkvPreItem) / 4);
+      PkvPreItem item;
+      item.row = ip[0];
+      item.pos = ip[1];
+      item.n = ip[2];
+      item.table = ip[3];
+      item.sp = ip[4];
+      item.wp = ip[5];
+      item.v0 = ip[6];
+      item.v1 = ip[7];
+      item.slot = ip[8];
+      const int rows = min(item.n, a.rows - item.row);
+      if (rows <= 0) continue;
+      const int h = head * REP + r;
+      const plan_t table = plan + item.table;
+      const gmem_t hbase = pool + (size_t)head * kPkvHeadBytes;
+      auto page_of = [&](int v) { return v < item.sp ? v : item.wp + (v - item.sp); };
+      const int last = item.pos + item.n - 1;      // the tile's last position
 
-    int lim[QS], behind[QS];   // the last visible key, the last one behind the window
-    u32x4 qf[QS][4][NT];
-    float m2[QS], mr[QS];
-    f32x4 o[QS][8], ls[QS];
-#pragma unroll
-    for (int qs = 0; qs < QS; ++qs) {
-      const int my = 16 * (QS * half + qs) + qr;
-      const bool ok = my < rows;
-      lim[qs] = ok ? item.pos + my : item.pos;   // rows past the end see what the first does
-      behind[qs] = a.window ? lim[qs] - a.window : -1;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks)
-        load_terms<A, NT>(a.q, ((size_t)(item.row + my) * nh + h) * HD + 32 * ks + 8 * kg, ok, qf[qs][ks]);
-      m2[qs] = -INFINITY;
-      mr[qs] = 0.f;
-      ls[qs] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int d = 0; d < 8; ++d) o[qs][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    const uint32_t one2 = pack2<F16>(1.f, 1.f);
-    const u32x4 ones = u32x4{one2, one2, one2, one2};
-
-    // Codes of chunk x of a page (x < 256: K, else V): token (x / 4) % 64, block x % 4.
-    u32x4 raw[CH];
-    int rsc[CH];
-    auto fetch = [&](int v) {
-      const gmem_t hp = hbase + (size_t)table[page_of(v)] * stride;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int x = i * NTH + tid, t = (x >> 2) & 63, b = x & 3;
-        raw[i] = *(gmem16_t)(hp + 16 * x);
-        rsc[i] = hp[x < 256 ? kPkvKs + 64 * b + 4 * (4 * (t >> 4) + (t & 3)) + ((t >> 2) & 3)
-                            : kPkvVs + 64 * b + t];
-      }
-    };
-    // Widened into LDS.  K's NaN scale makes the token's scores NaN; V's values
-    // are kept finite (they meet p = 0 of the rows that do not see the token),
-    // and what lies past the last visible token, which no one may have
-    // written, is 0.
-    auto stage = [&](int v, int buf) {
-      const int kb = page_of(v) * kPkvPage;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int x = i * NTH + tid, t = (x >> 2) & 63, b = x & 3;
-        const bool isv = x >= 256;
-        int byte = rsc[i];
-        if (isv && byte == 255) byte = 127;
-        const float sc = __builtin_bit_cast(float, (uint32_t)byte << 23);
-        if (kb + t > last) raw[i] = u32x4{0, 0, 0, 0};
-        uint16_t* row = (isv ? sV[buf] : sK[buf]) + t * HD;
-        const int sw = isv ? swv(t) : swk(t);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *(u32x4*)(row + (((4 * b + j) ^ sw) << 3)) = widen8<F16>(raw[i][j], sc);
-      }
-    };
-    fetch(item.v0);   // an item has a page at least
-    stage(item.v0, 0);
-    __syncthreads();
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    for (int v = item.v0, buf = 0; v < item.v1; ++v, buf ^= 1) {
-      const int after = min(v + 1, item.v1 - 1);   // the last page once more, so that no branch is needed
-      fetch(after);
-      const int kb = page_of(v) * kPkvPage;
-      const uint16_t* kbuf = sK[buf];
-      const uint16_t* vbuf = sV[buf];
-      // LDS reads go out a group ahead of the products that use them (a group is
-      // 8 products, 128 cycles; a read takes about as long): K by tile, V by
-      // half-block of tokens and half of the dims.  The scheduling barriers keep
-      // the compiler from pulling them back together.
-      f32x4 s[4][QS];
-      u32x4 kf[2][4];
-      auto read_k = [&](int mt) {
-        const int t = 16 * mt + qr;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-          kf[mt & 1][ks] = *(const u32x4*)(kbuf + t * HD + (((4 * ks + kg) ^ swk(t)) << 3));
-      };
-      s16x4 vf[2][4][2];
-      auto read_v = [&](int gr) {
-        const int t = 32 * (gr >> 1) + 4 * kg + (qr >> 2);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = 4 * (gr & 1) + i;
-          const uint16_t* at = vbuf + t * HD + (((2 * d + ((qr & 3) >> 1)) ^ swv(t)) << 3) + 4 * (qr & 1);
-          vf[gr & 1][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
-          vf[gr & 1][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * HD));
-        }
-      };
-      read_k(0);
-      __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        if (mt < 3) read_k(mt + 1);
-        else read_v(0);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int qs = 0; qs < QS; ++qs) s[mt][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-          for (int qs = 0; qs < QS; ++qs)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) s[mt][qs] = mfma<F16>(kf[mt & 1][ks], qf[qs][ks][n], s[mt][qs]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      __builtin_amdgcn_s_setprio(0);
-      const bool full = kb + kPkvPage - 1 <= item.pos &&
-                        (a.window == 0 || kb > last - a.window || kb + kPkvPage <= a.sinks);
-      bool grow = false;
-      float bm[QS];
+      int lim[QS], behind[QS];   // the last visible key, the last one behind the window
+      u32x4 qf[QS][4][NT];
+      float m2[QS], mr[QS];
+      f32x4 o[QS][8], ls[QS];
 #pragma unroll
       for (int qs = 0; qs < QS; ++qs) {
-        if (!full) {
+        const int my = 16 * (QS * half + qs) + qr;
+        const bool ok = my < rows;
+        lim[qs] = ok ? item.pos + my : item.pos;   // rows past the end see what the first does
+        behind[qs] = a.window ? lim[qs] - a.window : -1;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int j = kb + 16 * (e >> 2) + 4 * kg + (e & 3);
-            const bool hidden = (j > lim[qs]) | ((j <= behind[qs]) & (j >= a.sinks));
-            s[e >> 2][qs][e & 3] = hidden ? -INFINITY : s[e >> 2][qs][e & 3];
-          }
-        }
-        bm[qs] = s[0][qs][0];
+        for (int ks = 0; ks < 4; ++ks)
+          load_terms<A, NT>(a.q, ((size_t)(item.row + my) * nh + h) * HD + 32 * ks + 8 * kg, ok, qf[qs][ks]);
+        m2[qs] = -INFINITY;
+        mr[qs] = 0.f;
+        ls[qs] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 1; e < 16; ++e) bm[qs] = fmaxf(bm[qs], s[e >> 2][qs][e & 3]);
-        grow |= fmaf(bm[qs], c2, -mr[qs]) > kGrow || m2[qs] == -INFINITY;
+        for (int d = 0; d < 8; ++d) o[qs][d] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
-      if (__any(grow)) {
+      const uint32_t one2 = pack2<F16>(1.f, 1.f);
+      const u32x4 ones = u32x4{one2, one2, one2, one2};
+
+      // Codes of chunk x of a page (x < 256: K, else V): token (x / 4) % 64, block x % 4.
+      u32x4 raw[CH];
+      int rsc[CH];
+      auto fetch = [&](int v) {
+        const gmem_t hp = hbase + (size_t)table[page_of(v)] * stride;
 #pragma unroll
-        for (int qs = 0; qs < QS; ++qs) {
-          float x = fmaxf(bm[qs], __shfl_xor(bm[qs], 16));
-          x = fmaxf(x, __shfl_xor(x, 32));
-          const float mn = fmaxf(m2[qs], x * c2), nr = mn == -INFINITY ? 0.f : mn;
-          const float f = __builtin_amdgcn_exp2f(m2[qs] - nr);
-          m2[qs] = mn;
-          mr[qs] = nr;
-          ls[qs] *= f;
-#pragma unroll
-          for (int d = 0; d < 8; ++d) o[qs][d] *= f;
-        }
-      }
-      // O^T += V^T P^T over tokens 32 hb .. 32 hb + 31: k-slot i of group kg is
-      // token 32 hb + 4 kg + i (i < 4) or 32 hb + 16 + 4 kg + i - 4, where S^T has them
-      u32x4 pb[2][QS][NT];
-      auto weigh = [&](int hb, int qs) {
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const f32x4 x = s[2 * hb + (e >> 2)][qs];
-          float p0 = __builtin_amdgcn_exp2f(fmaf(x[e & 3], c2, -mr[qs]));
-          float p1 = __builtin_amdgcn_exp2f(fmaf(x[(e & 3) + 1], c2, -mr[qs]));
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            pb[hb][qs][n][e / 2] = pack2<F16>(p0, p1);
-            if (n + 1 < NT) {
-              p0 -= rd_bf16(p0);
-              p1 -= rd_bf16(p1);
-            }
-          }
+        for (int i = 0; i < CH; ++i) {
+          const int x = i * NTH + tid, t = (x >> 2) & 63, b = x & 3;
+          raw[i] = *(gmem16_t)(hp + 16 * x);
+          rsc[i] = hp[x < 256 ? kPkvKs + 64 * b + 4 * (4 * (t >> 4) + (t & 3)) + ((t >> 2) & 3)
+                              : kPkvVs + 64 * b + t];
         }
       };
+      // Widened into LDS.  K's NaN scale makes the token's scores NaN; V's values
+      // are kept finite (they meet p = 0 of the rows that do not see the token),
+      // and what lies past the last visible token, which no one may have
+      // written, is 0.
+      auto stage = [&](int v, int buf) {
+        const int kb = page_of(v) * kPkvPage;
 #pragma unroll
-      for (int qs = 0; qs < QS; ++qs) weigh(0, qs);
-      __builtin_amdgcn_s_setprio(1);
+        for (int i = 0; i < CH; ++i) {
+          const int x = i * NTH + tid, t = (x >> 2) & 63, b = x & 3;
+          const bool isv = x >= 256;
+          int byte = rsc[i];
+          if (isv && byte == 255) byte = 127;
+          const float sc = __builtin_bit_cast(float, (uint32_t)byte << 23);
+          if (kb + t > last) raw[i] = u32x4{0, 0, 0, 0};
+          uint16_t* row = (isv ? sV[buf] : sK[buf]) + t * HD;
+          const int sw = isv ? swv(t) : swk(t);
 #pragma unroll
-      for (int gr = 0; gr < 4; ++gr) {
-        const int hb = gr >> 1;
-        if (gr < 3) read_v(gr + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        if ((gr & 1) == 0) {
-#pragma unroll
-          for (int qs = 0; qs < QS; ++qs)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) ls[qs] = mfma<F16>(ones, pb[hb][qs][n], ls[qs]);
+          for (int j = 0; j < 4; ++j) *(u32x4*)(row + (((4 * b + j) ^ sw) << 3)) = widen8<F16>(raw[i][j], sc);
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = 4 * (gr & 1) + i;
-          const u32x4 va = __builtin_bit_cast(
-              u32x4, __builtin_shufflevector(vf[gr & 1][i][0], vf[gr & 1][i][1], 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int qs = 0; qs < QS; ++qs)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) o[qs][d] = mfma<F16>(va, pb[hb][qs][n], o[qs][d]);
-        }
-        // the second half's exponentials between the first half's products
-        if (gr < 2 && gr < QS) weigh(1, gr);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      __builtin_amdgcn_s_setprio(0);
-      stage(after, buf ^ 1);
+      };
+      fetch(item.v0);   // an item has a page at least
+      stage(item.v0, 0);
       __syncthreads();
-    }
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      for (int v = item.v0, buf = 0; v < item.v1; ++v, buf ^= 1) {
+        const int after = min(v + 1, item.v1 - 1);   // the last page once more, so that no branch is needed
+        fetch(after);
+        const int kb = page_of(v) * kPkvPage;
+        const uint16_t* kbuf = sK[buf];
+        const uint16_t* vbuf = sV[buf];
+        // LDS reads go out a group ahead of the products that use them (a group is
+        // 8 products, 128 cycles; a read takes about as long): K by tile, V by
+        // half-block of tokens and half of the dims.  The scheduling barriers keep
+        // the compiler from pulling them back together.
+        f32x4 s[4][QS];
+        u32x4 kf[2][4];
+        auto read_k = [&](int mt) {
+          const int t = 16 * mt + qr;
 #pragma unroll
-    for (int qs = 0; qs < QS; ++qs) {
-      const int my = 16 * (QS * half + qs) + qr;
-      if (my >= rows) continue;
-      if (item.slot < 0) {
-        const float inv = 1.f / ls[qs][0];
-        const size_t at = ((size_t)(item.row + my) * nh + h) * HD + 4 * kg;
+          for (int ks = 0; ks < 4; ++ks)
+            kf[mt & 1][ks] = *(const u32x4*)(kbuf + t * HD + (((4 * ks + kg) ^ swk(t)) << 3));
+        };
+        s16x4 vf[2][4][2];
+        auto read_v = [&](int gr) {
+          const int t = 32 * (gr >> 1) + 4 * kg + (qr >> 2);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const f32x4 x = o[qs][d] * inv;
-          if constexpr (A == ACT_F32) {
-            *(f32x4*)((float*)a.out + at + 16 * d) = x;
-          } else {
-            uint32_t* p = (uint32_t*)((uint16_t*)a.out + at + 16 * d);
-            p[0] = pack2<F16>(x[0], x[1]);
-            p[1] = pack2<F16>(x[2], x[3]);
+          for (int i = 0; i < 4; ++i) {
+            const int d = 4 * (gr & 1) + i;
+            const uint16_t* at = vbuf + t * HD + (((2 * d + ((qr & 3) >> 1)) ^ swv(t)) << 3) + 4 * (qr & 1);
+            vf[gr & 1][i][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+            vf[gr & 1][i][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * HD));
+          }
+        };
+        read_k(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          if (mt < 3) read_k(mt + 1);
+          else read_v(0);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) s[mt][qs] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) s[mt][qs] = mfma<F16>(kf[mt & 1][ks], qf[qs][ks][n], s[mt][qs]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        const bool full = kb + kPkvPage - 1 <= item.pos &&
+                          (a.window == 0 || kb > last - a.window || kb + kPkvPage <= a.sinks);
+        bool grow = false;
+        float bm[QS];
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) {
+          if (!full) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int j = kb + 16 * (e >> 2) + 4 * kg + (e & 3);
+              const bool hidden = (j > lim[qs]) | ((j <= behind[qs]) & (j >= a.sinks));
+              s[e >> 2][qs][e & 3] = hidden ? -INFINITY : s[e >> 2][qs][e & 3];
+            }
+          }
+          bm[qs] = s[0][qs][0];
+#pragma unroll
+          for (int e = 1; e < 16; ++e) bm[qs] = fmaxf(bm[qs], s[e >> 2][qs][e & 3]);
+          grow |= fmaf(bm[qs], c2, -mr[qs]) > kGrow || m2[qs] == -INFINITY;
+        }
+        if (__any(grow)) {
+#pragma unroll
+          for (int qs = 0; qs < QS; ++qs) {
+            float x = fmaxf(bm[qs], __shfl_xor(bm[qs], 16));
+            x = fmaxf(x, __shfl_xor(x, 32));
+            const float mn = fmaxf(m2[qs], x * c2), nr = mn == -INFINITY ? 0.f : mn;
+            const float f = __builtin_amdgcn_exp2f(m2[qs] - nr);
+            m2[qs] = mn;
+            mr[qs] = nr;
+            ls[qs] *= f;
+#pragma unroll
+            for (int d = 0; d < 8; ++d) o[qs][d] *= f;
           }
         }
-      } else {
-        const size_t u = ((size_t)item.slot * a.nkv + head) * (TP * REP) + my * REP + r;
+        // O^T += V^T P^T over tokens 32 hb .. 32 hb + 31: k-slot i of group kg is
+        // token 32 hb + 4 kg + i (i < 4) or 32 hb + 16 + 4 kg + i - 4, where S^T has them
+        u32x4 pb[2][QS][NT];
+        auto weigh = [&](int hb, int qs) {
 #pragma unroll
-        for (int d = 0; d < 8; ++d) *(f32x4*)(a.pre_o + u * HD + 16 * d + 4 * kg) = o[qs][d];
-        if (kg == 0) {
-          a.pre_ml[2 * u] = m2[qs];
-          a.pre_ml[2 * u + 1] = ls[qs][0];
+          for (int e = 0; e < 8; e += 2) {
+            const f32x4 x = s[2 * hb + (e >> 2)][qs];
+            float p0 = __builtin_amdgcn_exp2f(fmaf(x[e & 3], c2, -mr[qs]));
+            float p1 = __builtin_amdgcn_exp2f(fmaf(x[(e & 3) + 1], c2, -mr[qs]));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              pb[hb][qs][n][e / 2] = pack2<F16>(p0, p1);
+              if (n + 1 < NT) {
+                p0 -= rd_bf16(p0);
+                p1 -= rd_bf16(p1);
+              }
+            }
+          }
+        };
+#pragma unroll
+        for (int qs = 0; qs < QS; ++qs) weigh(0, qs);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int gr = 0; gr < 4; ++gr) {
+          const int hb = gr >> 1;
+          if (gr < 3) read_v(gr + 1);
+          __builtin_amdgcn_sched_barrier(0);
+          if ((gr & 1) == 0) {
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) ls[qs] = mfma<F16>(ones, pb[hb][qs][n], ls[qs]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = 4 * (gr & 1) + i;
+            const u32x4 va = __builtin_bit_cast(
+                u32x4, __builtin_shufflevector(vf[gr & 1][i][0], vf[gr & 1][i][1], 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+            for (int qs = 0; qs < QS; ++qs)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) o[qs][d] = mfma<F16>(va, pb[hb][qs][n], o[qs][d]);
+          }
+          // the second half's exponentials between the first half's products
+          if (gr < 2 && gr < QS) weigh(1, gr);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        stage(after, buf ^ 1);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int qs = 0; qs < QS; ++qs) {
+        const int my = 16 * (QS * half + qs) + qr;
+        if (my >= rows) continue;
+        if (item.slot < 0) {
+          const float inv = 1.f / ls[qs][0];
+          const size_t at = ((size_t)(item.row + my) * nh + h) * HD + 4 * kg;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            const f32x4 x = o[qs][d] * inv;
+            if constexpr (A == ACT_F32) {
+              *(f32x4*)((float*)a.out + at + 16 * d) = x;
+            } else {
+              uint32_t* p = (uint32_t*)((uint16_t*)a.out + at + 16 * d);
+              p[0] = pack2<F16>(x[0], x[1]);
+              p[1] = pack2<F16>(x[2], x[3]);
+            }
+          }
+        } else {
+          const size_t u = ((size_t)item.slot * a.nkv + head) * (TP * REP) + my * REP + r;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) *(f32x4*)(a.pre_o + u * HD + 16 * d + 4 * kg) = o[qs][d];
+          if (kg == 0) {
+            a.pre_ml[2 * u] = m2[qs];
+            a.pre_ml[2 * u + 1] = ls[qs][0];
+          }
         }
       }
-    }
-    __syncthreads();
+      __syncthreads();
     }
   }
 }
