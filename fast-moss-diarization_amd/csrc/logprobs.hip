@@ -20,7 +20,7 @@
 // work-group's waves have told each other, are looked at one by one.  Rows are
 // cut so that a launch has about kGroups work-groups; the last piece of a row to
 // end joins them all.
-// 1,000 rows of 151,936 bf16 logits (304 MB): 65-69 us, 4.6 TB/s, VALU issue about
+// 1,000 rows of 151,936 bf16 logits (304 MB): 64-69 us, 4.6 TB/s, VALU issue about
 // as long; with each wave's list on its own 73, with a search of the work-group
 // for each alternative and a barrier a tile 199.  8 f32 rows: 11.0-13.1 us alone
 // (the chain load -> statistics -> ticket -> join), among others 4.3-4.7 in some
